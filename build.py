@@ -17,7 +17,10 @@ OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libdm_hip.so")
 SOURCES = ["gemm.hip", "panel.hip", "ffn.hip", "attention.hip", "norm.hip", "elementwise.hip"]
 HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "panel.h"), os.path.join(ROOT, "include", "dm_hip.h")]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I" + os.path.join(ROOT, "include")]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler makes them from ordinary float code, and some of their forms have
+# given wrong results on MI355X now and then, without an error.  The host pass warns that it does not know the feature.
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I" + os.path.join(ROOT, "include"),
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target, deps):

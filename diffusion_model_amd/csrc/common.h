@@ -126,9 +126,7 @@ __device__ __forceinline__ float gelu_erf_fast_f(float x) {
     return fmaf(fabsf(h), erf_abs, h);           // 0.5 x (1 + sign(x) erf_abs)
 }
 
-// The same for two values at once, written on 2-vectors so that the multiply-adds compile to packed fp32 instructions
-// (v_pk_mul_f32 / v_pk_fma_f32: two lanes of arithmetic per issue slot); only the reciprocal and the exponential stay
-// scalar.  Bit-identical to two calls of gelu_erf_fast_f.
+// The same for two values at once, on 2-vectors.  Bit-identical to two calls of gelu_erf_fast_f.
 __device__ __forceinline__ f32x2 gelu_erf_fast_f2(f32x2 x) {
     const f32x2 ax = __builtin_elementwise_abs(x);
     const f32x2 w = ax * 0.84932180028801904272f;

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(512, 2) void ffn_geglu_kernel(FfnArgs p) {
         const float* const tb = tab + jt * 128 + fq * 16 + 4 * h + r;
         const f32x2 bv = *reinterpret_cast<const f32x2*>(tb), bg = *reinterpret_cast<const f32x2*>(tb + 8);
         const f32x2 cv = *reinterpret_cast<const f32x2*>(tb + 64), cg = *reinterpret_cast<const f32x2*>(tb + 64 + 8);
-        // LN(a) W^T = rstd * (a W'^T - mean * colsum(W')) + (beta W^T + b); two values per packed instruction
+        // LN(a) W^T = rstd * (a W'^T - mean * colsum(W')) + (beta W^T + b), two values at a time
         const f32x2 mu = {ln_mu[i], ln_mu[i]}, rs = {ln_rs[i], ln_rs[i]};
         const f32x2 gv = rs * (f32x2{acc[1][i][r], acc[1][i][r + 1]} - mu * cg) + bg;
         const f32x2 vv = rs * (f32x2{acc[0][i][r], acc[0][i][r + 1]} - mu * cv) + bv;

@@ -276,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void gemm_panel_kernel(PanelArgs p) {
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2) {
-                        // two values per packed instruction
+                        // two values at a time
                         const f32x2 g = gelu_erf_fast_f2(f32x2{acc[i][j + 2][r], acc[i][j + 2][r + 1]} + f32x2{bg[j][r], bg[j][r + 1]});
                         const f32x2 v = (f32x2{acc[i][j][r], acc[i][j][r + 1]} + f32x2{bv[j][r], bv[j][r + 1]}) * g;
                         o[4 * j + r] = v[0];
