@@ -15,8 +15,8 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "diffusion_model_amd", "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libdm_hip.so")
-SOURCES = ["gemm.hip", "panel.hip", "ffn.hip", "attention.hip", "norm.hip", "elementwise.hip"]
-HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "panel.h"), os.path.join(ROOT, "include", "dm_hip.h")]
+SOURCES = ["gemm.hip", "panel.hip", "ffn.hip", "attention.hip", "norm.hip", "elementwise.hip", "mx.hip", "mx_gemm.hip"]
+HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "panel.h"), os.path.join(CSRC, "mx.h"), os.path.join(ROOT, "include", "dm_hip.h")]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler makes them from ordinary float code, and some of their forms have
 # given wrong results on MI355X now and then, without an error.  The host pass warns that it does not know the feature.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I" + os.path.join(ROOT, "include"),
@@ -31,10 +31,11 @@ def _stale(target, deps):
 
 
 # The scheduler-step kernels promise separately rounded fp32 operations (bitwise equal to fp32
-# torch); hipcc's default would contract a*b+c into an FMA.
+# torch); hipcc's default would contract a*b+c into an FMA.  The row norms promise that a quantised result is the
+# quantisation of the fp32 one, whatever the storage type: no contraction that depends on the instantiation.
 # Attention reads its score accumulators with VALU every tile: keep MFMA results in VGPRs instead of
 # AGPRs (saves a v_accvgpr_read/write per value).
-EXTRA = {"elementwise.hip": ["-ffp-contract=off"],
+EXTRA = {"elementwise.hip": ["-ffp-contract=off"], "mx.hip": ["-ffp-contract=off"],
          "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

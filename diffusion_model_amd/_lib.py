@@ -13,6 +13,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DM_HIP_LIBRARY") or os.path.join(_HERE, "csrc", "libdm_hip.so")
 
 DM_F32, DM_BF16 = 0, 1
+DM_MXFP8, DM_MXFP4 = 8, 4  # microscaled formats (bits per value)
+NORM_RMS, NORM_LAYER = 0, 1
 EPI_PLAIN, EPI_GEGLU, EPI_NCHW_F32, EPI_QUICKGELU = 0, 1, 2, 3
 TILE_AUTO, TILE_128x128, TILE_64x128, TILE_64x64, TILE_256x128, TILE_32x64 = 0, 1, 2, 3, 4, 5
 (TILE_D128x128_S2, TILE_D128x128_S3, TILE_D256x128_S3, TILE_D64x128_S3, TILE_D64x128_S4, TILE_D64x64_S4,
@@ -93,6 +95,28 @@ class FfnDesc(C.Structure):
     ]
 
 
+class RowNormDesc(C.Structure):
+    """DmRowNormDesc: RMS / layer norm with the residual's addition and an optional MX output (dm_row_norm)."""
+    _fields_ = [
+        ("x", C.c_void_p), ("ldx", C.c_long), ("r", C.c_void_p), ("ldr", C.c_long), ("h", C.c_void_p), ("ldh", C.c_long),
+        ("gamma", C.c_void_p), ("beta", C.c_void_p),
+        ("y", C.c_void_p), ("ldy", C.c_long), ("y_scales", C.c_void_p), ("ldys", C.c_long),
+        ("rows", C.c_long), ("c", C.c_int), ("dtype", C.c_int), ("kind", C.c_int), ("out_fmt", C.c_int), ("eps", C.c_float),
+    ]
+
+
+class MxGemmDesc(C.Structure):
+    """DmMxGemmDesc: product of two microscaled matrices (dm_mx_gemm)."""
+    _fields_ = [
+        ("x", C.c_void_p), ("ldx", C.c_long), ("x_scales", C.c_void_p), ("ld_xs", C.c_long),
+        ("w", C.c_void_p), ("ldw", C.c_long), ("w_scales", C.c_void_p), ("ld_ws", C.c_long),
+        ("x_fmt", C.c_int), ("w_fmt", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+        ("bias", C.c_void_p), ("r", C.c_void_p), ("ldr", C.c_long),
+        ("c", C.c_void_p), ("ldc", C.c_long), ("c_scales", C.c_void_p), ("ld_cs", C.c_long),
+        ("c_type", C.c_int), ("epi", C.c_int),
+    ]
+
+
 _vp, _l, _i, _f = C.c_void_p, C.c_long, C.c_int, C.c_float
 _PROTOS = {
     "dm_abi_version": (C.c_int, []),
@@ -118,6 +142,10 @@ _PROTOS = {
     "dm_init": (C.c_int, []),
     "dm_groupnorm_noalloc": (C.c_int, [_vp, _l, _vp, _l, _i, _i, _i, _i, _i, _vp, _vp, _f, _i, _vp]),
     "dm_layernorm": (C.c_int, [_vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp]),
+    "dm_mx_quantize": (C.c_int, [_vp, _l, _l, _i, _i, _i, _vp, _l, _vp, _l, _vp]),
+    "dm_mx_dequantize": (C.c_int, [_vp, _l, _vp, _l, _l, _i, _i, _vp, _l, _i, _vp]),
+    "dm_row_norm": (C.c_int, [C.POINTER(RowNormDesc), _vp]),
+    "dm_mx_gemm": (C.c_int, [C.POINTER(MxGemmDesc), _vp]),
     "dm_attention": (C.c_int, [_vp, _l, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "dm_attention_split_f32": (C.c_int, [_vp, _l, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _i, _i, _i, _vp]),
     "dm_embed_tokens": (C.c_int, [_vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp]),
@@ -169,7 +197,7 @@ def lib() -> C.CDLL:
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        if handle.dm_abi_version() != 13:
+        if handle.dm_abi_version() != 14:
             raise RuntimeError("libdm_hip.so ABI version mismatch; rebuild with `python build.py`")
         _lib = handle
     return _lib

@@ -1,0 +1,335 @@
+// Quantisation to the microscaled (MX) formats and back, and the row norms (RMS / layer norm with the residual's addition)
+// that write them.  All of it is bound by HBM: every value is read once, with 16-byte accesses where rows are aligned.
+#include "dm_hip.h"
+#include "mx.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+// Eight consecutive values at p, of which those below `left` exist (the others read as zero).
+template <typename T> __device__ __forceinline__ void load8(const T* p, int left, bool vec, float* v) {
+    constexpr int EPC = ElemTraits<T>::EPC;
+    if (vec) {  // left is 8 or more, or nothing exists
+#pragma unroll
+        for (int c = 0; c < 8 / EPC; ++c) chunk_to_f32<T>(ldg16(p + c * EPC, left >= 8), v + c * EPC);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? ElemTraits<T>::load(p + i) : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, int left, bool vec, const float* v) {
+    constexpr int EPC = ElemTraits<T>::EPC;
+    if (vec) {
+        if (left >= 8) {
+#pragma unroll
+            for (int c = 0; c < 8 / EPC; ++c) *reinterpret_cast<u32x4*>(p + c * EPC) = f32_to_chunk<T>(v + c * EPC);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) ElemTraits<T>::store(p + i, v[i]);
+    }
+}
+
+// ---- quantise / dequantise ------------------------------------------------------------------------------------------
+// A lane holds eight values, a quad the 32 of a block.  `gpr` = groups of eight per padded row (a multiple of 16), so a
+// quad never straddles rows; a block sweeps UNROLL x 256 consecutive groups with all its loads ahead of the arithmetic.
+constexpr int UNROLL = 4;
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(THREADS) void mx_quantize_kernel(const T* __restrict__ x, long ldx, long total, int gpr, int k, bool vec,
+                                                               unsigned char* __restrict__ codes, long ldc,
+                                                               unsigned char* __restrict__ scales, long lds) {
+    const long first = (long)blockIdx.x * (THREADS * UNROLL);
+    const long row0 = first / gpr;
+    const int g0 = (int)(first - row0 * gpr);
+    float v[UNROLL][8];
+    long row[UNROLL];
+    int g[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned at = g0 + u * THREADS + threadIdx.x;
+        const unsigned r = at / (unsigned)gpr;
+        row[u] = row0 + r;
+        g[u] = at - r * gpr;
+        if (first + u * THREADS + threadIdx.x < total) load8<T>(x + row[u] * ldx + g[u] * 8, k - g[u] * 8, vec, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+        if (first + u * THREADS + threadIdx.x < total)
+            mx_store_quad<FMT>(v[u], codes + row[u] * ldc + g[u] * mx_bytes(FMT, 8), scales + row[u] * lds + (g[u] >> 2), threadIdx.x);
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(THREADS) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, long ldc,
+                                                                 const unsigned char* __restrict__ scales, long lds, long total, int gpr,
+                                                                 int k, bool vec, T* __restrict__ y, long ldy) {
+    const long first = (long)blockIdx.x * (THREADS * UNROLL);
+    const long row0 = first / gpr;
+    const int g0 = (int)(first - row0 * gpr);
+    uint32_t w[UNROLL][2], s[UNROLL];
+    long row[UNROLL];
+    int g[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const unsigned at = g0 + u * THREADS + threadIdx.x;
+        const unsigned r = at / (unsigned)gpr;
+        row[u] = row0 + r;
+        g[u] = at - r * gpr;
+        if (first + u * THREADS + threadIdx.x < total) {
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(codes + row[u] * ldc + g[u] * mx_bytes(FMT, 8));
+            if constexpr (FMT == 8) {
+                const u32x2 t = *reinterpret_cast<const u32x2*>(p);
+                w[u][0] = t[0];
+                w[u][1] = t[1];
+            } else {
+                w[u][0] = p[0];
+            }
+            s[u] = scales[row[u] * lds + (g[u] >> 2)];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+        if (first + u * THREADS + threadIdx.x < total) {
+            float v[8];
+            mx_decode8<FMT>(w[u], mx_scale(s[u]), v);
+            store8<T>(y + row[u] * ldy + g[u] * 8, k - g[u] * 8, vec, v);
+        }
+}
+
+// ---- norms ----------------------------------------------------------------------------------------------------------
+struct NormArgs {
+    const void* x;
+    const void* r;  // residual or NULL
+    void* h;        // x + r (with r)
+    const float* gamma;
+    const float* beta;  // layer norm; NULL = none
+    void* y;            // T rows, or codes
+    unsigned char* ys;  // scales
+    long ldx, ldr, ldh, ldy, ldys;
+    long rows;
+    int c, layer;
+    float eps;
+    bool vec;
+};
+
+// Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    if constexpr (TPR > 64) {
+        __syncthreads();  // the previous sum has been read
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v += red[i];
+    }
+    return v;
+}
+// eight values of h = x + r, rounded to the storage type (the norm is that of the stored row)
+template <typename T> __device__ __forceinline__ void load_h(const NormArgs& p, long row, int at, float* v) {
+    load8<T>(static_cast<const T*>(p.x) + row * p.ldx + at, p.c - at, p.vec, v);
+    if (p.r) {
+        float r[8];
+        load8<T>(static_cast<const T*>(p.r) + row * p.ldr + at, p.c - at, p.vec, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] += r[i];
+            if constexpr (sizeof(T) == 2) v[i] = bf16_to_f32(f32_to_bf16(v[i]));
+        }
+    }
+}
+template <typename T, int OUT> __device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, float rstd) {
+    float w[8], o[8];
+    load8<float>(p.gamma + at, p.c - at, p.vec, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (v[i] - mean) * rstd * w[i];
+    if (p.beta) {
+        load8<float>(p.beta + at, p.c - at, p.vec, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += w[i];
+    }
+    if constexpr (OUT == 0) {
+        store8<T>(static_cast<T*>(p.y) + row * p.ldy + at, p.c - at, p.vec, o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = at + i < p.c ? o[i] : 0.f;
+        mx_store_quad<OUT>(o, static_cast<unsigned char*>(p.y) + row * p.ldy + mx_bytes(OUT, at), p.ys + row * p.ldys + (at >> 5), threadIdx.x);
+    }
+}
+
+// The row stays in registers: TPR threads of NV groups of eight values, so x and the residual are read once, and the layer
+// norm's variance is a second sum over registers, not a difference of moments.
+template <typename T, int OUT, int TPR, int NV>
+__global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
+    __shared__ float red[TPR / 64];
+    const int t = threadIdx.x % TPR;
+    const long row = (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+    if (row >= p.rows) return;  // whole waves; TPR > 64 has one row per block
+    const int cp = OUT ? mx_padded(p.c) : p.c;
+    float v[NV][8];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) load_h<T>(p, row, (n * TPR + t) * 8, v[n]);
+    float s = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int at = (n * TPR + t) * 8;
+        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, p.vec, v[n]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += p.layer ? v[n][i] : v[n][i] * v[n][i];
+    }
+    s = row_sum<TPR>(s, red) / p.c;
+    float mean = 0.f;
+    if (p.layer) {
+        mean = s;
+        s = 0.f;
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = (n * TPR + t) * 8 + i < p.c ? v[n][i] - mean : 0.f;
+                s = fmaf(d, d, s);
+            }
+        s = row_sum<TPR>(s, red) / p.c;
+    }
+    const float rstd = 1.f / sqrtf(s + p.eps);
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+        if ((n * TPR + t) * 8 < cp) norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, rstd);
+}
+
+// Rows too long for registers: one block per row sweeps it once per sum and once for the output; the sweeps behind the
+// first are served by the caches.  With a residual they read the stored h (each thread what it wrote itself), so h may be x
+// or the residual itself here as in the kernel above.
+template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_norm_loop_kernel(NormArgs p) {
+    __shared__ float red[THREADS / 64];
+    const long row = blockIdx.x;
+    const int cp = OUT ? mx_padded(p.c) : p.c;
+    const T* stored = p.r ? static_cast<const T*>(p.h) + row * p.ldh : static_cast<const T*>(p.x) + row * p.ldx;
+    float s = 0.f, mean = 0.f;
+    for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
+        float v[8];
+        load_h<T>(p, row, at, v);
+        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, p.vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += p.layer ? v[i] : v[i] * v[i];
+    }
+    s = row_sum<THREADS>(s, red) / p.c;
+    if (p.layer) {
+        mean = s;
+        s = 0.f;
+        for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
+            float v[8];
+            load8<T>(stored + at, p.c - at, p.vec, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = at + i < p.c ? v[i] - mean : 0.f;
+                s = fmaf(d, d, s);
+            }
+        }
+        s = row_sum<THREADS>(s, red) / p.c;
+    }
+    const float rstd = 1.f / sqrtf(s + p.eps);
+    for (int at = threadIdx.x * 8; at < cp; at += THREADS * 8) {
+        float v[8];
+        load8<T>(stored + at, p.c - at, p.vec, v);
+        norm_store<T, OUT>(p, row, at, v, mean, rstd);
+    }
+}
+
+template <typename T, int OUT, int TPR, int NV> int launch_row_norm(const NormArgs& p, hipStream_t s) {
+    row_norm_kernel<T, OUT, TPR, NV><<<dim3((unsigned)((p.rows + THREADS / TPR - 1) / (THREADS / TPR))), THREADS, 0, s>>>(p);
+    return dm_check_launch();
+}
+template <typename T, int OUT> int launch_norm(const NormArgs& p, hipStream_t s) {
+    if (p.c <= 512) return launch_row_norm<T, OUT, 64, 1>(p, s);
+    if (p.c <= 1024) return launch_row_norm<T, OUT, 64, 2>(p, s);
+    if (p.c <= 2048) return launch_row_norm<T, OUT, 256, 1>(p, s);
+    if (p.c <= 4096) return launch_row_norm<T, OUT, 256, 2>(p, s);
+    if (p.c <= 8192) return launch_row_norm<T, OUT, 256, 4>(p, s);
+    if (p.c <= 16384) return launch_row_norm<T, OUT, 256, 8>(p, s);
+    row_norm_loop_kernel<T, OUT><<<dim3((unsigned)p.rows), THREADS, 0, s>>>(p);
+    return dm_check_launch();
+}
+
+bool mx_fmt_ok(int fmt) { return fmt == DM_MXFP8 || fmt == DM_MXFP4; }
+bool dtype_ok(int dtype) { return dtype == DM_F32 || dtype == DM_BF16; }
+int esize(int dtype) { return dtype == DM_F32 ? 4 : 2; }
+bool rows_vec(const void* p, long ld, int esz) { return dm_aligned16(p) && (ld * esz) % 16 == 0; }
+// codes / scales of `rows` rows of k values: 0 or an error code
+int mx_layout(const void* codes, long ldc, const void* scales, long lds, int k, int fmt) {
+    if (!codes || !scales || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
+    const int kp = mx_padded(k);
+    if (ldc < mx_bytes(fmt, kp) || lds < kp / MX_BLOCK) return DM_ERR_ARG;
+    if (!dm_aligned16(codes) || ldc % 16 || (reinterpret_cast<uintptr_t>(scales) & 3u) || lds % 4) return DM_ERR_ALIGN;
+    return DM_OK;
+}
+constexpr int MAX_K = 1 << 24;       // values of a row: 32-bit offsets inside a row
+constexpr long MAX_GRID = 0x7fffffffL;
+
+}  // namespace
+
+extern "C" int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dtype, int fmt, unsigned char* codes, long ldc,
+                              unsigned char* scales, long lds, hipStream_t stream) {
+    if (rows < 0 || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
+    if (rows == 0) return DM_OK;
+    if (!x || ldx < k) return DM_ERR_ARG;
+    if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
+    const int gpr = mx_padded(k) / 8;
+    const long total = rows * gpr, blocks = (total + THREADS * UNROLL - 1) / (THREADS * UNROLL);
+    if (blocks > MAX_GRID) return DM_ERR_ARG;
+    const bool vec = k % 8 == 0 && rows_vec(x, ldx, esize(dtype));
+    const dim3 grid((unsigned)blocks);
+#define DM_MX_Q(T, F) \
+    mx_quantize_kernel<T, F><<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), ldx, total, gpr, k, vec, codes, ldc, scales, lds)
+    if (dtype == DM_F32) { if (fmt == DM_MXFP8) DM_MX_Q(float, 8); else DM_MX_Q(float, 4); }
+    else { if (fmt == DM_MXFP8) DM_MX_Q(bf16_t, 8); else DM_MX_Q(bf16_t, 4); }
+#undef DM_MX_Q
+    return dm_check_launch();
+}
+
+extern "C" int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsigned char* scales, long lds, long rows, int k, int fmt,
+                                void* y, long ldy, int dtype, hipStream_t stream) {
+    if (rows < 0 || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
+    if (rows == 0) return DM_OK;
+    if (!y || ldy < k) return DM_ERR_ARG;
+    if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
+    const int gpr = mx_padded(k) / 8;
+    const long total = rows * gpr, blocks = (total + THREADS * UNROLL - 1) / (THREADS * UNROLL);
+    if (blocks > MAX_GRID) return DM_ERR_ARG;
+    const bool vec = k % 8 == 0 && rows_vec(y, ldy, esize(dtype));
+    const dim3 grid((unsigned)blocks);
+#define DM_MX_D(T, F) \
+    mx_dequantize_kernel<T, F><<<grid, THREADS, 0, stream>>>(codes, ldc, scales, lds, total, gpr, k, vec, static_cast<T*>(y), ldy)
+    if (dtype == DM_F32) { if (fmt == DM_MXFP8) DM_MX_D(float, 8); else DM_MX_D(float, 4); }
+    else { if (fmt == DM_MXFP8) DM_MX_D(bf16_t, 8); else DM_MX_D(bf16_t, 4); }
+#undef DM_MX_D
+    return dm_check_launch();
+}
+
+extern "C" int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream) {
+    if (!d || d->rows < 0 || d->c < 1 || d->c > MAX_K || !dtype_ok(d->dtype) || (d->kind != DM_NORM_RMS && d->kind != DM_NORM_LAYER) ||
+        (d->out_fmt != 0 && !mx_fmt_ok(d->out_fmt)))
+        return DM_ERR_ARG;
+    if (d->rows == 0) return DM_OK;
+    if (!d->x || !d->gamma || !d->y || (d->r == nullptr) != (d->h == nullptr)) return DM_ERR_ARG;
+    const int esz = esize(d->dtype);
+    if (d->ldx < d->c || (d->r && (d->ldr < d->c || d->ldh < d->c)) || d->rows > MAX_GRID) return DM_ERR_ARG;
+    if (d->out_fmt) {
+        if (const int rc = mx_layout(d->y, d->ldy, d->y_scales, d->ldys, d->c, d->out_fmt)) return rc;
+    } else if (d->ldy < d->c) {
+        return DM_ERR_ARG;
+    }
+    NormArgs p;
+    p.x = d->x; p.r = d->r; p.h = d->h; p.gamma = d->gamma; p.beta = d->beta; p.y = d->y; p.ys = d->y_scales;
+    p.ldx = d->ldx; p.ldr = d->ldr; p.ldh = d->ldh; p.ldy = d->ldy; p.ldys = d->ldys;
+    p.rows = d->rows; p.c = d->c; p.layer = d->kind == DM_NORM_LAYER; p.eps = d->eps;
+    p.vec = d->c % 8 == 0 && rows_vec(d->x, d->ldx, esz) && (!d->r || (rows_vec(d->r, d->ldr, esz) && rows_vec(d->h, d->ldh, esz))) &&
+            dm_aligned16(d->gamma) && (!d->beta || dm_aligned16(d->beta)) && (d->out_fmt || rows_vec(d->y, d->ldy, esz));
+#define DM_NORM(T) \
+    (d->out_fmt == 0 ? launch_norm<T, 0>(p, stream) : d->out_fmt == DM_MXFP8 ? launch_norm<T, 8>(p, stream) : launch_norm<T, 4>(p, stream))
+    return d->dtype == DM_F32 ? DM_NORM(float) : DM_NORM(bf16_t);
+#undef DM_NORM
+}

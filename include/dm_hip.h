@@ -27,10 +27,14 @@
 extern "C" {
 #endif
 
-#define DM_ABI_VERSION 13
+#define DM_ABI_VERSION 14
 
 #define DM_F32 0
 #define DM_BF16 1
+/* Microscaled (MX) formats: 32 consecutive values of a row share the scale 2^(byte - 127); the values are e4m3 (largest 448)
+ * or e2m1 (largest 6, two to a byte, the even one in the low nibble). */
+#define DM_MXFP8 8
+#define DM_MXFP4 4
 
 #define DM_EPI_PLAIN 0    /* C = acc (+bias) (+rowbias[batch]) (+R) */
 #define DM_EPI_GEGLU 1    /* C[m][n] = (acc_v + b_v) * gelu_erf(acc_g + b_g), N counts both halves */
@@ -289,6 +293,67 @@ int dm_softmax_rows(void* x, long ld, int rows, int cols, float scale, int dtype
 /* LayerNorm over the channel dimension of [rows][c].  Replaces nn.LayerNorm (blocks.py:137,143,149). */
 int dm_layernorm(const void* x, long ldx, void* y, long ldy, int rows, int c, int dtype,
                  const float* gamma, const float* beta, float eps, hipStream_t stream);
+
+/* Microscaled (MX) operands; inference of networks whose Linear layers (attention.py:19-20,51-54; blocks.py:109-110;
+ * clip.py:76-88) run on 4- or 8-bit values.  No counterpart in the reference, which computes in fp32.
+ * A matrix of `rows` rows of k values is held as `codes` (rows of ldc bytes) and `scales` (rows of lds bytes).  Rows are padded
+ * to kp = k rounded up to 128: kp bytes (DM_MXFP8) or kp/2 bytes (DM_MXFP4) of codes and kp/32 scale bytes.  The padding of
+ * the codes must be zero; every entry point here that writes such a matrix writes its padding.  codes 16-byte aligned, ldc a
+ * multiple of 16; scales 4-byte aligned, lds a multiple of 4.
+ * Quantisation of a block of 32 values: byte = max(0, biased exponent of the largest magnitude - 8 (MXFP8) or 2 (MXFP4)); a
+ * value v becomes v * 2^(127 - byte) rounded to the nearest code, ties to even, saturated at the largest; a block that holds
+ * an infinity or a NaN gets byte 255 and zero codes and stands for NaN.
+ * x: rows of ldx fp32 / bf16 elements, any alignment (16-byte aligned rows with k a multiple of 8 are read 16 bytes at a time). */
+int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dtype, int fmt, unsigned char* codes, long ldc,
+                   unsigned char* scales, long lds, hipStream_t stream);
+/* The values that the codes stand for, as fp32 or bf16 (exact in both wherever the value is not a subnormal of the type). */
+int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsigned char* scales, long lds, long rows, int k, int fmt,
+                     void* y, long ldy, int dtype, hipStream_t stream);
+
+/* Norm of rows with the residual's addition in front and, optionally, quantisation behind it, in one pass:
+ *   h = x + r (rounded to dtype and stored; without r: h = x, nothing stored)
+ *   DM_NORM_RMS:   y = h / sqrt(mean(h^2) + eps) * gamma (+ beta)
+ *   DM_NORM_LAYER: y = (h - mean(h)) / sqrt(var(h) + eps) * gamma (+ beta)     (blocks.py:137,143,149; clip.py:99,110)
+ * y: rows of ldy elements of dtype (out_fmt 0), or an MX matrix of c values per row (out_fmt DM_MXFP8 / DM_MXFP4: y = codes,
+ * ldy bytes; y_scales, ldys).  Statistics in fp32.  r and h go together and are rows of dtype; h may be x or r itself, and y may
+ * be x when there is no quantisation.  Any row length up to 2^24 and any alignment. */
+#define DM_NORM_RMS 0
+#define DM_NORM_LAYER 1
+typedef struct DmRowNormDesc {
+    const void* x; long ldx;
+    const void* r; long ldr;
+    void* h; long ldh;
+    const float* gamma;
+    const float* beta;
+    void* y; long ldy;
+    unsigned char* y_scales; long ldys;
+    long rows;
+    int c, dtype, kind, out_fmt;
+    float eps;
+} DmRowNormDesc;
+int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream);
+
+/* Product of two MX matrices, C = act(X W^T + bias) + r: X m x k, W n x k (both formats, in any combination).
+ * epi: DM_EPI_PLAIN, DM_EPI_QUICKGELU, or DM_EPI_GEGLU (rows 0 .. n/2 of W are the values, the others the gates; n even; C has
+ * n/2 columns).  bias: n fp32 or NULL.  c_type: DM_BF16 / DM_F32 (rows of ldc elements; r, optional, has the same type), or
+ * DM_MXFP8 / DM_MXFP4 (c = codes, ldc bytes; c_scales, ld_cs; no r): an MX matrix ready to be the next product's X.
+ * Accumulation in fp32.  DM_BF16 and MX results come from the scaled matrix instructions on the codes themselves, whose adder
+ * drops low bits of e4m3 products (2e-5 of the result on normal data); DM_F32 results with an e4m3 operand from bf16 matrix instructions on
+ * the decoded operands, which are exact there. */
+typedef struct DmMxGemmDesc {
+    const unsigned char* x; long ldx;
+    const unsigned char* x_scales; long ld_xs;
+    const unsigned char* w; long ldw;
+    const unsigned char* w_scales; long ld_ws;
+    int x_fmt, w_fmt;
+    int m, n, k;
+    const float* bias;
+    const void* r; long ldr;
+    void* c; long ldc;
+    unsigned char* c_scales; long ld_cs;
+    int c_type, epi;
+} DmMxGemmDesc;
+int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream);
 
 /* softmax(q k^T / sqrt(d)) v for all heads, never materialising the score matrix.
  * Replaces attention.py:34-43 (self; causal != 0 adds the upper-triangular mask of attention.py:35-37,
