@@ -15,8 +15,15 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "diffusion_model_amd", "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libdm_hip.so")
-SOURCES = ["gemm.hip", "panel.hip", "ffn.hip", "attention.hip", "norm.hip", "elementwise.hip", "mx.hip", "mx_gemm.hip"]
-HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "panel.h"), os.path.join(CSRC, "mx.h"), os.path.join(ROOT, "include", "dm_hip.h")]
+SOURCES = ["gemm.hip", "panel.hip", "ffn.hip", "attention.hip", "norm.hip", "elementwise.hip", "mx.hip", "mx_gemm.hip", "mx_split.hip"]
+HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "panel.h"), os.path.join(ROOT, "include", "dm_hip.h")]
+MX_HEADERS = [os.path.join(CSRC, "mx.h"), os.path.join(CSRC, "mx_gemm.h")]
+
+
+def _deps(src):
+    return [os.path.join(CSRC, src), *HEADERS, *(MX_HEADERS if src.startswith("mx") else [])]
+
+
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler makes them from ordinary float code, and some of their forms have
 # given wrong results on MI355X now and then, without an error.  The host pass warns that it does not know the feature.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I" + os.path.join(ROOT, "include"),
@@ -60,7 +67,7 @@ def build_variant(tag: str, defines) -> str:
     objs = []
     for src in SOURCES:
         obj = os.path.join(obj_dir, src.replace(".hip", ".o"))
-        if _stale(obj, [os.path.join(CSRC, src), *HEADERS]):
+        if _stale(obj, _deps(src)):
             subprocess.run(["hipcc", *FLAGS, *defines, *EXTRA.get(src, []), "-c", os.path.join(CSRC, src), "-o", obj], check=True)
         objs.append(obj)
     lib = os.path.join(CSRC, f"libdm_hip_{tag}.so")
@@ -75,9 +82,9 @@ def build_timeline() -> str:
 def build(force: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
-    todo = [s for s, o in zip(SOURCES, objs) if force or _stale(o, [os.path.join(CSRC, s), *HEADERS])]
+    todo = [s for s, o in zip(SOURCES, objs) if force or _stale(o, _deps(s))]
     if todo:
-        with ThreadPoolExecutor(max_workers=min(4, len(todo))) as ex:
+        with ThreadPoolExecutor(max_workers=min(8, len(todo))) as ex:
             list(ex.map(_compile, todo))
     if todo or _stale(LIB, objs):
         subprocess.run(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs], check=True)

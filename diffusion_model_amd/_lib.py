@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("DM_HIP_LIBRARY") or os.path.join(_HERE, "csrc", "libd
 DM_F32, DM_BF16 = 0, 1
 DM_MXFP8, DM_MXFP4 = 8, 4  # microscaled formats (bits per value)
 NORM_RMS, NORM_LAYER = 0, 1
+X_MX, X_BF16, X_F32, X_ROWS_MAX_M = 0, 1, 2, 16  # what DmMxGemmDesc.x points at
 EPI_PLAIN, EPI_GEGLU, EPI_NCHW_F32, EPI_QUICKGELU = 0, 1, 2, 3
 TILE_AUTO, TILE_128x128, TILE_64x128, TILE_64x64, TILE_256x128, TILE_32x64 = 0, 1, 2, 3, 4, 5
 (TILE_D128x128_S2, TILE_D128x128_S3, TILE_D256x128_S3, TILE_D64x128_S3, TILE_D64x128_S4, TILE_D64x64_S4,
@@ -110,7 +111,7 @@ class MxGemmDesc(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("ldx", C.c_long), ("x_scales", C.c_void_p), ("ld_xs", C.c_long),
         ("w", C.c_void_p), ("ldw", C.c_long), ("w_scales", C.c_void_p), ("ld_ws", C.c_long),
-        ("x_fmt", C.c_int), ("w_fmt", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+        ("x_fmt", C.c_int), ("w_fmt", C.c_int), ("x_src", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
         ("bias", C.c_void_p), ("r", C.c_void_p), ("ldr", C.c_long),
         ("c", C.c_void_p), ("ldc", C.c_long), ("c_scales", C.c_void_p), ("ld_cs", C.c_long),
         ("c_type", C.c_int), ("epi", C.c_int),

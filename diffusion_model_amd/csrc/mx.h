@@ -13,45 +13,53 @@ __host__ __device__ constexpr int mx_emax(int fmt) { return fmt == 8 ? 8 : 2; }
 __host__ __device__ constexpr int mx_bytes(int fmt, int values) { return fmt == 8 ? values : values / 2; }
 __host__ __device__ constexpr int mx_padded(int k) { return (k + MX_PAD - 1) / MX_PAD * MX_PAD; }
 
-// Magnitudes compare as unsigned integers, and a NaN's pattern exceeds infinity's: one integer maximum finds the block's
-// largest magnitude and whether anything in it is not finite (a float maximum would drop the NaN).
-__device__ __forceinline__ uint32_t mx_abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-template <int FMT> __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top_bits) {
-    const uint32_t e = top_bits >> 23;  // biased; 0 for zero and for subnormals, whose scale is the smallest one anyway
-    return e == 255u ? 255u : (e > (uint32_t)mx_emax(FMT) ? e - mx_emax(FMT) : 0u);
+// Largest magnitude of N values; NaN if one of them is (v_maximum3_f32 passes a NaN on, v_max_f32 would drop it).
+template <int N> __device__ __forceinline__ float mx_largest(const float* v) {
+    float top = __builtin_fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(v[i]), __builtin_fabsf(v[i + 1])), top);
+    if constexpr (N % 2 == 0) top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[N - 1]));
+    return top;
 }
-// 2^-(byte - 127): a normal number for every byte that mx_scale_byte gives but 255
-__device__ __forceinline__ float mx_inverse_scale(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
+template <int FMT> __device__ __forceinline__ uint32_t mx_scale_byte(float top) {
+    const uint32_t e = __float_as_uint(top) >> 23;  // biased (the sign is 0); 0 for zero and subnormals, whose scale is the smallest anyway
+    return (e & 255u) == 255u ? 255u : (e > (uint32_t)mx_emax(FMT) ? e - mx_emax(FMT) : 0u);
+}
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : (byte == 0u ? 0x00400000u : byte << 23));
 }
 
-// Eight values times `inv` -> eight codes in W words (W = 2: e4m3, 1: e2m1); round to nearest even.  The product is exact
-// (a power of two) except where it underflows far below half the smallest code.
+// Eight values -> eight codes in W words (W = 2: e4m3, 1: e2m1) under the scale 2^(byte - 127); to nearest even, saturated; zeros
+// under byte 255.  The conversions divide by the scale themselves (exactly, a power of two; 2^-127 included) and the 4-bit one
+// saturates; the 8-bit one makes NaN of what is too large, hence the clamp.
 template <int FMT> struct MxCodes {
     static constexpr int W = FMT == 8 ? 2 : 1;
     uint32_t w[W];
 };
-template <int FMT> __device__ __forceinline__ MxCodes<FMT> mx_encode8(const float* v, float inv, bool finite) {
+template <int FMT> __device__ __forceinline__ MxCodes<FMT> mx_encode8(const float* v, uint32_t byte) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const float scale = mx_scale(byte);
     MxCodes<FMT> c;
     if constexpr (FMT == 8) {
+        const float most = 448.f * scale;
         float u[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.f, 448.f);  // the conversion itself does not saturate
+        for (int i = 0; i < 8; ++i) u[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * h], u[4 * h + 1], 0, false);
-            c.w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * h + 2], u[4 * h + 3], w, true);
+            s16x2 w = {0, 0};
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, u[4 * h], u[4 * h + 1], scale, false);
+            c.w[h] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, u[4 * h + 2], u[4 * h + 3], scale, true));
         }
     } else {
-        uint32_t w = 0;  // saturates by itself
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0] * inv, v[1] * inv, 1.0f, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * inv, v[3] * inv, 1.0f, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4] * inv, v[5] * inv, 1.0f, 2);
-        c.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6] * inv, v[7] * inv, 1.0f, 3);
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+        c.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
     }
 #pragma unroll
-    for (int i = 0; i < MxCodes<FMT>::W; ++i) c.w[i] = finite ? c.w[i] : 0u;
+    for (int i = 0; i < MxCodes<FMT>::W; ++i) c.w[i] = byte == 255u ? 0u : c.w[i];
     return c;
 }
 template <int FMT> __device__ __forceinline__ void mx_decode8(const uint32_t* w, float scale, float* v) {
@@ -75,17 +83,14 @@ template <int FMT> __device__ __forceinline__ void mx_decode8(const uint32_t* w,
     }
 }
 // largest of the four lanes of a quad (the 32 values of a block when every lane holds eight)
-__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));  // quad_perm 1 0 3 2
-    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // quad_perm 2 3 0 1
+__device__ __forceinline__ float mx_quad_largest(float v) {
+    v = __builtin_elementwise_maximum(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true)));  // quad_perm 1 0 3 2
+    return __builtin_elementwise_maximum(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, true)));  // 2 3 0 1
 }
 // A quad's 32 values -> codes and (first lane) scale.  `codes` points at this lane's eight codes, `scale` at the block's byte.
 template <int FMT> __device__ __forceinline__ void mx_store_quad(const float* v, unsigned char* codes, unsigned char* scale, int lane) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, mx_abs_bits(v[i]));
-    const uint32_t byte = mx_scale_byte<FMT>(mx_quad_max(top));
-    const MxCodes<FMT> c = mx_encode8<FMT>(v, mx_inverse_scale(byte), byte != 255u);
+    const uint32_t byte = mx_scale_byte<FMT>(mx_quad_largest(mx_largest<8>(v)));
+    const MxCodes<FMT> c = mx_encode8<FMT>(v, byte);
     if constexpr (FMT == 8) *reinterpret_cast<u32x2*>(codes) = u32x2{c.w[0], c.w[1]};
     else *reinterpret_cast<uint32_t*>(codes) = c.w[0];
     if ((lane & 3) == 0) *scale = (unsigned char)byte;

@@ -5,28 +5,9 @@
 // W is the instruction's first operand, so that a lane holds 16 columns of C for one row; the rows of a 32-row W fragment are
 // permuted when they are brought to LDS such that those 16 columns follow each other (and lanes l, l + 32 hold the 32 columns of
 // an MX block of C).
-#include "dm_hip.h"
-#include "mx.h"
+#include "mx_gemm.h"
 
 namespace {
-
-typedef __attribute__((ext_vector_type(8))) int i32x8;
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-
-struct MxArgs {
-    const unsigned char *x, *xs, *w, *ws;
-    long ldx, ld_xs, ldw, ld_ws;
-    int m, n_out, n_pad;  // rows of C; columns of C; columns to write (MX results: padded, the padding as zeros)
-    int nkt;              // k-tiles of 128 values
-    int tiles_m, tiles_n;
-    const float* bias;
-    const void* r;
-    void* c;
-    unsigned char* cs;
-    long ldr, ldc, ld_cs;
-    int epi, c_type;
-    bool vec;             // rows of C and r may be accessed 16 bytes at a time
-};
 
 // Also waits for this wave's LDS reads: what follows is the barrier behind which other waves refill what they read.
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
@@ -55,68 +36,63 @@ __device__ __forceinline__ void to_lds4(const unsigned char* src, unsigned char*
 template <int F> __device__ __forceinline__ int swizzle(int row, int chunk) {
     return F == 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
 }
-template <int F> __device__ __forceinline__ u32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
-    return *reinterpret_cast<const u32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F>(row, chunk) * 16);
+template <int F> __device__ __forceinline__ i32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
+    return *reinterpret_cast<const i32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F>(row, chunk) * 16);
 }
-template <int F> __device__ __forceinline__ i32x8 lds_fragment(const unsigned char* base, int row, int g, int j) {
-    u32x4 lo, hi = {0u, 0u, 0u, 0u};
+// EXACT: both formats as the plain block 2 g + j, for products in bf16.
+template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type lds_fragment(const unsigned char* base, int row, int g, int j) {
     if constexpr (F == 8) {
-        lo = lds_chunk<8>(base, row, 2 * j + g);
-        hi = lds_chunk<8>(base, row, 2 * (2 + j) + g);
+        const i32x4 lo = lds_chunk<8>(base, row, EXACT ? 2 * (2 * g + j) : 2 * j + g);
+        const i32x4 hi = lds_chunk<8>(base, row, EXACT ? 2 * (2 * g + j) + 1 : 2 * (2 + j) + g);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-        lo = lds_chunk<4>(base, row, 2 * g + j);
-    }
-    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-}
-// The same block, decoded to bf16 with its scale applied (exact: at most four significant bits): 32 values in four chunks.
-template <int F> __device__ __forceinline__ void lds_fragment_bf16(const unsigned char* base, int row, int g, int j, float scale, u32x4* out) {
-    if constexpr (F == 8) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const u32x4 c = lds_chunk<8>(base, row, 2 * (2 * g + j) + h);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float v[8];
-                const uint32_t w[2] = {c[2 * q], c[2 * q + 1]};
-                mx_decode8<8>(w, scale, v);
-                out[2 * h + q] = f32_to_chunk<bf16_t>(v);
-            }
-        }
-    } else {
-        const u32x4 c = lds_chunk<4>(base, row, 2 * g + j);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float v[8];
-            const uint32_t w[1] = {c[q]};
-            mx_decode8<4>(w, scale, v);
-            out[q] = f32_to_chunk<bf16_t>(v);
-        }
+        return lds_chunk<4>(base, row, 2 * g + j);
     }
 }
-template <int WF, int XF, int J> __device__ __forceinline__ f32x16 mma_scaled(const i32x8& w, const i32x8& x, const f32x16& acc, int sw, int sx) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc, WF == 8 ? 0 : 4, XF == 8 ? 0 : 4, J, sw, J, sx);
+// Half J of a k-tile: one X fragment with every W fragment.
+template <int XF, int WF, bool EXACT, int J, int FN>
+__device__ __forceinline__ void mma_row(f32x16 (&acc)[FN], const typename MxFragment<XF>::type& x, const typename MxFragment<WF>::type (&w)[FN],
+                                        int sx, const int (&sw)[FN]) {
+    if constexpr (!EXACT) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(w[j]), widen(x), acc[j], WF == 8 ? 0 : 4, XF == 8 ? 0 : 4, J, sw[j], J, sx);
+    } else {
+        u32x4 xb[4];
+        decode_block<XF>(x, mx_scale((sx >> (8 * J)) & 255), xb);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            u32x4 wb[4];
+            decode_block<WF>(w[j], mx_scale((sw[j] >> (8 * J)) & 255), wb);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, wb[q]), __builtin_bit_cast(bf16x8, xb[q]), acc[j], 0, 0, 0);
+        }
+    }
 }
 
 // ---- epilogue --------------------------------------------------------------------------------------------------------
-// 16 consecutive columns of row m from column `col` on (values past n_out are zeros already) in the result's type.
-__device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float* v, int lane) {
+// 16 consecutive columns of row m from column `col` on, in the result's type; `edge`: some of the block's are past n_out.
+template <int F> __device__ __forceinline__ void store16_mx(const MxArgs& p, long m, int col, const float* v, int lane) {
+    // lanes l and l + 32 hold the two halves of a block
+    float top = mx_largest<16>(v);
+    top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32));
+    if (m >= p.m || col >= p.n_pad) return;
+    const uint32_t byte = mx_scale_byte<F>(top);
+    const MxCodes<F> a = mx_encode8<F>(v, byte), b = mx_encode8<F>(v + 8, byte);
+    unsigned char* dst = static_cast<unsigned char*>(p.c) + m * p.ldc + mx_bytes(F, col);
+    if constexpr (F == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{a.w[0], a.w[1], b.w[0], b.w[1]};
+    else *reinterpret_cast<u32x2*>(dst) = u32x2{a.w[0], b.w[0]};
+    if (lane < 32) p.cs[m * p.ld_cs + (col >> 5)] = (unsigned char)byte;
+}
+__device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float* v, int lane, bool edge) {
     if (p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4) {
-        // lanes l and l + 32 hold the two halves of a block
-        uint32_t top = 0;
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = max(top, mx_abs_bits(v[i]));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-        if (m >= p.m || col >= p.n_pad) return;
-        const uint32_t byte = p.c_type == DM_MXFP8 ? mx_scale_byte<8>(top) : mx_scale_byte<4>(top);
-        const float inv = mx_inverse_scale(byte);
-        if (p.c_type == DM_MXFP8) {
-            const MxCodes<8> a = mx_encode8<8>(v, inv, byte != 255u), b = mx_encode8<8>(v + 8, inv, byte != 255u);
-            *reinterpret_cast<u32x4*>(static_cast<unsigned char*>(p.c) + m * p.ldc + col) = u32x4{a.w[0], a.w[1], b.w[0], b.w[1]};
-        } else {
-            const MxCodes<4> a = mx_encode8<4>(v, inv, byte != 255u), b = mx_encode8<4>(v + 8, inv, byte != 255u);
-            *reinterpret_cast<u32x2*>(static_cast<unsigned char*>(p.c) + m * p.ldc + (col >> 1)) = u32x2{a.w[0], b.w[0]};
+            for (int e = 0; e < 16; ++e) v[e] = col + e < p.n_out ? v[e] : 0.f;
         }
-        if (lane < 32) p.cs[m * p.ld_cs + (col >> 5)] = (unsigned char)byte;
+        if (p.c_type == DM_MXFP8) store16_mx<8>(p, m, col, v, lane);
+        else store16_mx<4>(p, m, col, v, lane);
         return;
     }
     if (m >= p.m || col >= p.n_out) return;
@@ -158,24 +134,28 @@ __device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float*
         }
     }
 }
-__device__ __forceinline__ void load_bias16(const MxArgs& p, int at, int left, float* b) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = p.bias && i < left ? p.bias[at + i] : 0.f;
-}
-
 // ---- tile kernel -----------------------------------------------------------------------------------------------------
 // BM rows of X by BN rows of W per block, one WM x WN piece per wave; a ring of STAGES k-tiles in LDS, filled by loads that
 // bypass the registers.  EXACT: the operands are decoded to bf16 and multiplied there (see dm_mx_gemm).
+//
+// Scales would cost a request as many cache lines as it has lanes if they were fetched per k-tile (four bytes of every row; measured
+// at 8192^3, 4 bits: a fifth of the kernel's time).  They are fetched for a group of four k-tiles, 16 bytes of a row, a
+// quarter of the tile's rows with every k-tile: "quarter" q = 4 group + c is requested with k-tile q - 3 and is used with k-tile 4
+// group at the earliest, when every request up to that k-tile's has landed.
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> struct MxTile {
     static constexpr int XB = mx_bytes(XF, MX_PAD), WB = mx_bytes(WF, MX_PAD);
     static constexpr int WAVES = (BM / WM) * (BN / WN);
-    static constexpr int STAGE = BM * XB + BN * WB + (BM + BN) * 4;  // bytes
-    static constexpr int NX = BM * XB / 1024, NW = BN * WB / 1024, NS = (BM + BN) / 64;  // requests of a wave's 64 lanes per k-tile
-    static constexpr int PX = (NX + WAVES - 1) / WAVES, PW = (NW + WAVES - 1) / WAVES, PS = (NS + WAVES - 1) / WAVES;
-    static constexpr int LOADS = PX + PW + PS;  // per wave; where a kind does not divide, waves repeat a request (same bytes)
+    static constexpr int STAGE = BM * XB + BN * WB;  // bytes
+    // A group's first quarter is requested STAGES + 3 k-tiles ahead of the group; with two stages the group two before it has
+    // been read by then, with more the third before it.
+    static constexpr int GROUPS = STAGES > 2 ? 3 : 2, GROUP = (BM + BN) * 16;
+    static constexpr int LDS = STAGES * STAGE + GROUPS * GROUP;
+    static constexpr int PX = BM * XB / 1024 / WAVES, PW = BN * WB / 1024 / WAVES;  // requests of a wave's 64 lanes per k-tile
+    static constexpr int LOADS = PX + PW + 1;
     static_assert(BM % 64 == 0 && BN % 64 == 0 && WM % 32 == 0 && WN % 32 == 0, "whole requests and fragments");
+    static_assert(PX * WAVES * 1024 == BM * XB && PW * WAVES * 1024 == BN * WB && BM == BN && (BM + BN) / 64 <= WAVES, "every wave requests the same");
     static_assert(WN % 64 == 0, "a wave holds both the values and the gates of its columns");
-    static_assert((STAGES - 1) * LOADS <= 63, "vmcnt counts to 63");
+    static_assert((STAGES - 1) * LOADS <= 63 && STAGES >= 2 && STAGES <= 4, "vmcnt counts to 63");
 };
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES>
@@ -187,154 +167,227 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     const int wm = wave % (BM / WM), wn = wave / (BM / WM);
     const bool geglu = p.epi == DM_EPI_GEGLU;
 
-    const int tile_m = blockIdx.x % p.tiles_m, tile_n = blockIdx.x / p.tiles_m;
+    // Blocks go to the 8 XCDs in turn and each XCD has its own L2: give an XCD a run of neighbouring tiles, walked down
+    // GROUP_M tile rows before the next tile column, so that its 32 CUs share a patch of 8 x 4 tiles' operands.
+    int tile_m, tile_n;
+    {
+        constexpr int XCDS = 8, GROUP_M = 8;
+        const int nb = gridDim.x, xcd = blockIdx.x % XCDS, per = nb / XCDS, more = nb % XCDS;
+        const int t = xcd * per + min(xcd, more) + blockIdx.x / XCDS;
+        const int in_group = GROUP_M * p.tiles_n, group = t / in_group, rest = t - group * in_group;
+        const int rows = min(GROUP_M, p.tiles_m - group * GROUP_M);
+        tile_m = group * GROUP_M + rest % rows;
+        tile_n = rest / rows;
+    }
     const int m0 = tile_m * BM;
     const int col0 = tile_n * (geglu ? BN / 2 : BN);  // first column of C
 
-    // ---- sources of this wave's requests.  Rows that do not exist are read from row m - 1 / the last row and not stored.
-    const unsigned char *xp[G::PX], *wp[G::PW], *sp[G::PS];
-    int xd[G::PX], wd[G::PW], sd[G::PS];
-    auto w_row = [&](int rho) {  // row of W behind LDS row rho of the tile
+    // ---- sources of this wave's requests: a scalar base that moves on by a k-tile, and each lane's offset from it.  A request
+    // lies inside one 32-row W fragment, so values and gates have bases of their own and no offset spans the matrix.  Rows
+    // that do not exist are read from the last one and their products not stored.
+    const unsigned char* xbase = p.x + (long)m0 * p.ldx;
+    const int first = min(col0, p.n_out - 1);  // col0 can lie in the padding of an MX result
+    const unsigned char* wbase = p.w + (long)first * p.ldw;
+    const long gate_bytes = geglu ? p.n_out * p.ldw : 0;
+    const int rows_left = p.m - 1 - m0, cols_left = p.n_out - 1 - first;
+    uint32_t xo[G::PX], wo[G::PW];
+    auto w_col = [&](int rho) {  // column of the tile behind LDS row rho
         const int f = rho >> 5, i = rho & 31;
-        const int col = 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
-        const int o = col0 + (geglu ? (f >> 1) : f) * 32 + col;
-        return (long)min(o, p.n_out - 1) + (geglu && (f & 1) ? p.n_out : 0);
+        return min((geglu ? f >> 1 : f) * 32 + 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3), cols_left);
     };
+    auto gate = [&](int rho) { return geglu && ((rho >> 5) & 1); };
 #pragma unroll
     for (int i = 0; i < G::PX; ++i) {
-        const int slot = (wave + i * G::WAVES) % G::NX;
-        const int row = slot * (1024 / G::XB) + lane / (G::XB / 16), pos = lane % (G::XB / 16);
-        xp[i] = p.x + (long)min(m0 + row, p.m - 1) * p.ldx + swizzle<XF>(row, pos) * 16;
-        xd[i] = slot * 1024;
+        const int row = (wave + i * G::WAVES) * (1024 / G::XB) + lane / (G::XB / 16), pos = lane % (G::XB / 16);
+        xo[i] = (uint32_t)min(row, rows_left) * (uint32_t)p.ldx + swizzle<XF>(row, pos) * 16;
     }
 #pragma unroll
     for (int i = 0; i < G::PW; ++i) {
-        const int slot = (wave + i * G::WAVES) % G::NW;
-        const int row = slot * (1024 / G::WB) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
-        wp[i] = p.w + w_row(row) * p.ldw + swizzle<WF>(row, pos) * 16;
-        wd[i] = BM * G::XB + slot * 1024;
+        const int row = (wave + i * G::WAVES) * (1024 / G::WB) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
+        wo[i] = (uint32_t)w_col(row) * (uint32_t)p.ldw + swizzle<WF>(row, pos) * 16;
     }
-#pragma unroll
-    for (int i = 0; i < G::PS; ++i) {
-        const int slot = (wave + i * G::WAVES) % G::NS;
-        const int row = slot * 64 + lane;
-        sp[i] = row < BM ? p.xs + (long)min(m0 + row, p.m - 1) * p.ld_xs : p.ws + w_row(row - BM) * p.ld_ws;
-        sd[i] = BM * G::XB + BN * G::WB + slot * 256;
-    }
+    // scalar base + 32-bit lane offset in every request: hidden from the optimiser, which would make each a 64-bit address of its
+    // own, carried and advanced in two more registers
+    auto lane_offset = [](uint32_t o) { asm volatile("" : "+v"(o)); return o; };
     auto request = [&](int stage) {
         unsigned char* base = smem + stage * G::STAGE;
 #pragma unroll
-        for (int i = 0; i < G::PX; ++i) { to_lds16(xp[i], base + xd[i]); xp[i] += G::XB; }
+        for (int i = 0; i < G::PX; ++i) to_lds16(xbase + lane_offset(xo[i]), base + (wave + i * G::WAVES) * 1024);
 #pragma unroll
-        for (int i = 0; i < G::PW; ++i) { to_lds16(wp[i], base + wd[i]); wp[i] += G::WB; }
-#pragma unroll
-        for (int i = 0; i < G::PS; ++i) { to_lds4(sp[i], base + sd[i]); sp[i] += 4; }
+        for (int i = 0; i < G::PW; ++i) {
+            const int slot = wave + i * G::WAVES;
+            to_lds16(wbase + (gate(slot * (1024 / G::WB)) ? gate_bytes : 0) + lane_offset(wo[i]), base + BM * G::XB + slot * 1024);
+        }
+        xbase += G::XB;
+        wbase += G::WB;
+    };
+
+    // quarter q = 4 group + c: rows c (BM + BN) / 4 .. of the group's buffer [row][16 bytes], 16 rows per wave and four lanes per
+    // row (a second set of waves repeats the first's); c = 0, 1 are rows of X, 2, 3 rows of W.  Computed without a branch or an indexed register: the loop below is one block.
+    unsigned char* const scales = smem + STAGES * G::STAGE;
+    constexpr int QUARTER = (BM + BN) / 4;
+    const int qwave = wave % (QUARTER / 16), qrow = qwave * 16 + (lane >> 2);
+    const uint32_t xs0 = (uint32_t)min(qrow, rows_left) * (uint32_t)p.ld_xs, xs1 = (uint32_t)min(QUARTER + qrow, rows_left) * (uint32_t)p.ld_xs;
+    const uint32_t ws0 = (uint32_t)w_col(qrow) * (uint32_t)p.ld_ws, ws1 = (uint32_t)w_col(QUARTER + qrow) * (uint32_t)p.ld_ws;
+    const uint32_t xs_odd = xs0 ^ xs1, ws_odd = ws0 ^ ws1;
+    const uint64_t xscales = (uint64_t)(p.xs + (long)m0 * p.ld_xs), wscales = (uint64_t)(p.ws + (long)first * p.ld_ws);
+    const uint64_t gate_scales = geglu ? (uint64_t)(p.n_out * p.ld_ws) : 0;
+    int quarter = 0, fill = 0;  // next quarter to request and its group's buffer
+    const int last_kt = p.nkt - 1;
+    auto request_scales = [&]() {
+        const uint32_t odd = quarter & 1, of_w = (quarter >> 1) & 1;
+        const uint32_t is_gate = ((odd * QUARTER + qwave * 16) >> 5) & 1;
+        const uint64_t wsrc = wscales + (gate_scales & (0 - (uint64_t)is_gate));
+        const uint64_t src = xscales ^ ((xscales ^ wsrc) & (0 - (uint64_t)of_w));
+        const uint32_t xoff = xs0 ^ (xs_odd & (0 - odd)), woff = ws0 ^ (ws_odd & (0 - odd));
+        const uint32_t at = 4 * min((quarter & ~3) + (lane & 3), last_kt);  // quarters behind the last k-tile repeat it, unread
+        to_lds4((const unsigned char*)src + ((xoff ^ ((xoff ^ woff) & (0 - of_w))) + at), scales + fill * G::GROUP + ((quarter & 3) * QUARTER + qwave * 16) * 16);
+        if ((++quarter & 3) == 0) fill = fill + 1 == G::GROUPS ? 0 : fill + 1;
     };
 
     constexpr int FM = WM / 32, FN = WN / 32;
+    // a lane's 16 columns of W fragment j begin at `col`; the sums start from the bias
     f32x16 acc[FM][FN];
+    auto column = [&](int j) { return geglu ? col0 + wn * (WN / 2) + (j >> 1) * 32 + 16 * g : col0 + wn * WN + j * 32 + 16 * g; };
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < FN; ++j) {
+        f32x16 b = {};
+        if (p.bias) {
+            const int col = column(j), left = p.n_out - col;
+            const float* src = p.bias + (geglu && (j & 1) ? p.n_out : 0) + col;
+            if (col0 + (geglu ? BN / 2 : BN) <= p.n_out) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
-
+                for (int e = 0; e < 16; ++e) b[e] = src[e];
+            } else {
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
-        if (s < p.nkt) request(s);
-    int stage = 0;
-    for (int kt = 0; kt < p.nkt; ++kt) {
-        // k-tile kt has landed once only younger requests are outstanding; behind the barrier it is visible to all waves and
-        // all reads of the stage that is refilled next are done
-        wait_young<G::LOADS, STAGES - 2>(p.nkt - 1 - kt);
-        __builtin_amdgcn_s_barrier();
-        if (kt + STAGES - 1 < p.nkt) request(stage == 0 ? STAGES - 1 : stage - 1);
-        const unsigned char* xb = smem + stage * G::STAGE;
-        const unsigned char* wb = xb + BM * G::XB;
-        const unsigned char* sb = wb + BN * G::WB;
-        int sx[FM], sw[FN];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) sx[i] = *reinterpret_cast<const uint16_t*>(sb + (wm * WM + i * 32 + fr) * 4 + 2 * g);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) sw[j] = *reinterpret_cast<const uint16_t*>(sb + (BM + wn * WN + j * 32 + fr) * 4 + 2 * g);
-        if constexpr (!EXACT) {
-#define MX_HALF(J)                                                                                                              \
-    {                                                                                                                           \
-        i32x8 xf[FM], wf[FN];                                                                                                   \
-        _Pragma("unroll") for (int i = 0; i < FM; ++i) xf[i] = lds_fragment<XF>(xb, wm * WM + i * 32 + fr, g, J);                \
-        _Pragma("unroll") for (int j = 0; j < FN; ++j) wf[j] = lds_fragment<WF>(wb, wn * WN + j * 32 + fr, g, J);                \
-        _Pragma("unroll") for (int i = 0; i < FM; ++i)                                                                          \
-            _Pragma("unroll") for (int j = 0; j < FN; ++j) acc[i][j] = mma_scaled<WF, XF, J>(wf[j], xf[i], acc[i][j], sw[j], sx[i]); \
-    }
-            MX_HALF(0)
-            MX_HALF(1)
-#undef MX_HALF
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4 xf[FM][4], wf[FN][4];
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-                    lds_fragment_bf16<XF>(xb, wm * WM + i * 32 + fr, g, h, mx_scale((sx[i] >> (8 * h)) & 255), xf[i]);
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    lds_fragment_bf16<WF>(wb, wn * WN + j * 32 + fr, g, h, mx_scale((sw[j] >> (8 * h)) & 255), wf[j]);
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, wf[j][q]),
-                                                                                __builtin_bit_cast(bf16x8, xf[i][q]), acc[i][j], 0, 0, 0);
+                for (int e = 0; e < 16; ++e) b[e] = e < left ? src[e] : 0.f;
             }
         }
-        if (++stage == STAGES) stage = 0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][j] = b;
     }
 
-    // ---- epilogue: lane holds row m0 + .. + fr, 16 columns per fragment
+    // ---- k loop.  A k-tile is two halves of FM x FN matrix instructions.  X fragment i of the next half is read from LDS as
+    // soon as the instructions on X fragment i of this one have been issued; W fragments, which all of them use, have two sets.
+    // The wait and the barrier for the next k-tile stand behind the first instructions of the second half: every wave has read
+    // all of this k-tile by then, so its stage is refilled at once, and the matrix pipe has work meanwhile.
+    typename MxFragment<XF>::type x[FM];
+    typename MxFragment<WF>::type w[2][FN];
+    int sx[FM], sw[FN], sx_next[FM], sw_next[FN];
+    const int xrow = wm * WM + fr, wrow = wn * WN + fr;
+    auto read_x = [&](int stage, int half, int i) { x[i] = lds_fragment<XF, EXACT>(smem + stage * G::STAGE, xrow + i * 32, g, half); };
+    auto read_w = [&](int stage, int half) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) w[half][j] = lds_fragment<WF, EXACT>(smem + stage * G::STAGE + BM * G::XB, wrow + j * 32, g, half);
+    };
+    int next = 0, drain = 0;  // k-tile whose scales are read next and its group's buffer
+    auto read_scales = [&]() {
+        const unsigned char* sb = scales + drain * G::GROUP + (next & 3) * 4 + 2 * g;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sx_next[i] = *reinterpret_cast<const uint16_t*>(sb + (xrow + i * 32) * 16);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sw_next[j] = *reinterpret_cast<const uint16_t*>(sb + (BM + wrow + j * 32) * 16);
+        if ((++next & 3) == 0) drain = drain + 1 == G::GROUPS ? 0 : drain + 1;
+    };
+
+    for (int q = 0; q < STAGES + 3; ++q) request_scales();
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+        if (s < p.nkt) request(s);
+    wait_young<G::LOADS - 1, STAGES - 1>(p.nkt - 1);
+    __builtin_amdgcn_s_barrier();
+    read_scales();
+    read_w(0, 0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) read_x(0, 0, i);
+    constexpr int BARRIER_AT = FM >= 4 ? 1 : 0;
+    int stage = 0;
+    // LEFT: k-tiles behind this one that have been requested, STAGES - 1 at most; MORE: one more is requested into this one's
+    // stage.  Both are constants and the body has no branch, so the order below is the order of issue.  (Requests spread
+    // between the matrix instructions instead of issued together: no difference at 8192^3, and spills for 8-bit operands.)
+    auto k_tile = [&](auto left, auto more) {
+        constexpr int LEFT = decltype(left)::value;
+        constexpr bool MORE = decltype(more)::value;
+        const int here = stage;
+        if (++stage == STAGES) stage = 0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sx[i] = sx_next[i];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sw[j] = sw_next[j];
+        read_w(here, 1);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            mma_row<XF, WF, EXACT, 0>(acc[i], x[i], w[0], sx[i], sw);
+            read_x(here, 1, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            mma_row<XF, WF, EXACT, 1>(acc[i], x[i], w[1], sx[i], sw);
+            if constexpr (LEFT > 0) {
+                if (i == BARRIER_AT) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    wait_vm<(LEFT - 1) * (G::LOADS - 1)>();  // requests of scales among the younger ones only make it wait for more
+                    __builtin_amdgcn_s_barrier();
+                    if constexpr (MORE) {
+                        request_scales();
+                        request(here);
+                    }
+                    read_scales();
+                    read_w(stage, 0);
+#pragma unroll
+                    for (int e = 0; e < BARRIER_AT; ++e) read_x(stage, 0, e);
+                }
+                if (i >= BARRIER_AT) read_x(stage, 0, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int left = p.nkt - 1;
+    for (; left >= STAGES; --left) k_tile(std::integral_constant<int, STAGES - 1>(), std::true_type());
+    if constexpr (STAGES > 3)
+        if (left >= 3) { k_tile(std::integral_constant<int, 3>(), std::false_type()); --left; }
+    if constexpr (STAGES > 2)
+        if (left >= 2) { k_tile(std::integral_constant<int, 2>(), std::false_type()); --left; }
+    if (left >= 1) k_tile(std::integral_constant<int, 1>(), std::false_type());
+    k_tile(std::integral_constant<int, 0>(), std::false_type());
+
+    // ---- epilogue: a lane holds row .. + fr and 16 columns per fragment
+    const bool edge = col0 + (geglu ? BN / 2 : BN) > p.n_out;
     if (geglu) {
 #pragma unroll
-        for (int j = 0; j < FN / 2; ++j) {
-            const int col = col0 + wn * (WN / 2) + j * 32 + 16 * g, left = p.n_out - col;
-            float bv[16], bg[16];
-            load_bias16(p, col, left, bv);
-            load_bias16(p, p.n_out + col, left, bg);
+        for (int j = 0; j < FN; j += 2)
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 float v[16];
+                if (p.c_type == DM_F32) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float gate = acc[i][2 * j + 1][e] + bg[e];
-                    const float o = (acc[i][2 * j][e] + bv[e]) * (p.c_type == DM_F32 ? gelu_erf_f(gate) : gelu_erf_fast_f(gate));
-                    v[e] = e < left ? o : 0.f;
+                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_erf_f(acc[i][j + 1][e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_erf_fast_f(acc[i][j + 1][e]);
                 }
-                store16(p, m0 + wm * WM + i * 32 + fr, col, v, lane);
+                store16(p, m0 + wm * WM + i * 32 + fr, column(j), v, lane, edge);
             }
-        }
     } else {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int col = col0 + wn * WN + j * 32 + 16 * g, left = p.n_out - col;
-            float b[16];
-            load_bias16(p, col, left, b);
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 float v[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float o = acc[i][j][e] + b[e];
-                    if (p.epi == DM_EPI_QUICKGELU) o = o / (1.f + __expf(-1.702f * o));
-                    v[e] = e < left ? o : 0.f;
+                    const float o = acc[i][j][e];
+                    v[e] = p.epi == DM_EPI_QUICKGELU ? o / (1.f + __expf(-1.702f * o)) : o;
                 }
-                store16(p, m0 + wm * WM + i * 32 + fr, col, v, lane);
+                store16(p, m0 + wm * WM + i * 32 + fr, column(j), v, lane, edge);
             }
-        }
     }
 }
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {
     typedef MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES> G;
-    constexpr int LDS = STAGES * G::STAGE;
+    constexpr int LDS = G::LDS;
     static DmLdsAttr attr;
     const void* fn = reinterpret_cast<const void*>(&mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES>);
     if (LDS > 64 * 1024)
@@ -346,18 +399,56 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }
+// Which tile: measured over m = 1 .. 16384, n, k = 320, 1280, 5120 and 8192^2 (e4m3 x e2m1, bf16 result).
+//   256 x 256  one block per CU; 1.1 to 1.3 times the rate of the next where its rounds over the 256 CUs are full
+//              (16384 x 5120 x 5120: 343 us against 414; 4096 x 5120 x 5120, 1.25 rounds: 131 against 109)
+//   128 x 128  two blocks per CU; with waves of 32 x 64 below ten k-tiles, where the epilogue's latency counts
+//              (16384 x 5120 x 320: 63 us against 71), of 64 x 64 above (4096 x 5120 x 5120: 109 against 113)
+//   64 x 64    while the 128 x 128 tiles do not fill the chip twice, or once for a long k
+//              (1024 x 5120 x 1280: 14.0 us against 14.8; 1024 x 1280 x 5120: 22.7 against 27.8, x 5120 x 5120: 46 against 39)
 template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_t s) {
-    return launch<XF, WF, EXACT, 64, 64, 32, 64, 3>(p, s);
+    const int wide = p.epi == DM_EPI_GEGLU ? 2 * p.n_pad : p.n_pad;
+    auto tiles = [&](int t) { return (long)((p.m + t - 1) / t) * ((wide + t - 1) / t); };
+    if constexpr (!EXACT) {
+        const long t256 = tiles(256), rounds = (t256 + 255) / 256;
+        if (t256 * 5 >= rounds * 256 * 4) return launch<XF, WF, EXACT, 256, 256, 128, 64, XF == 4 && WF == 4 ? 3 : 2>(p, s);
+    }
+    const long t128 = tiles(128);
+    if (t128 >= 512 || (t128 >= 256 && p.nkt >= 20)) {
+        if (p.nkt < 10 || EXACT) return launch<XF, WF, EXACT, 128, 128, 32, 64, 2>(p, s);
+        return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
+    }
+    return launch<XF, WF, EXACT, 64, 64, 32, 64, 2>(p, s);
 }
-template <int XF, int WF> int launch_type(const MxArgs& p, hipStream_t s) {
+template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream_t s) {
     if constexpr (XF == 8 || WF == 8)
-        if (p.c_type == DM_F32) return launch_fmt<XF, WF, true>(p, s);
+        if (exact) return launch_fmt<XF, WF, true>(p, s);
     return launch_fmt<XF, WF, false>(p, s);
 }
+// The split kernel's tile: the smallest that needs at most one block per CU, since blocks read their operands anew
+// (64 x 1280 x 5120: 10.6 us in 320 blocks, 8.2 in 160; 16 x 8192 x 8192: 15.7 in 512, 11.7 in 256, the tile kernel 29).  Up to
+// 16 rows it is taken at any size: W is read once then, and that is all there is to do.
+bool split_tile(const MxArgs& p, int* fm, int* fn) {
+    static const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {1, 4}};
+    const bool geglu = p.epi == DM_EPI_GEGLU, mx = p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4;
+    for (const auto& t : shapes) {
+        const int cols = geglu ? t[1] * 8 : t[1] * 16;
+        if ((geglu && t[1] % 2) || (mx && cols % MX_BLOCK) || (t[0] > 1 && p.m <= 16)) continue;
+        const long blocks = (long)((p.m + 16 * t[0] - 1) / (16 * t[0])) * ((p.n_pad + cols - 1) / cols);
+        if (blocks <= 256 || (p.m <= 16 && t[1] == 4)) {
+            *fm = t[0];
+            *fn = t[1];
+            return true;
+        }
+    }
+    return false;
+}
 
+constexpr long MAX_LD = 1L << 24;  // bytes of a row: 32-bit offsets inside the rows of a tile
 bool fmt_ok(int fmt) { return fmt == DM_MXFP8 || fmt == DM_MXFP4; }
 int operand(const void* codes, long ld, const void* scales, long lds, int kp, int fmt) {
     if (!codes || !scales || ld < mx_bytes(fmt, kp) || lds < kp / MX_BLOCK) return DM_ERR_ARG;
+    if (ld > MAX_LD || lds > MAX_LD) return DM_ERR_ARG;
     return dm_aligned16(codes) && ld % 16 == 0 && !(reinterpret_cast<uintptr_t>(scales) & 3u) && lds % 4 == 0 ? DM_OK : DM_ERR_ALIGN;
 }
 
@@ -370,10 +461,14 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
     if (d->c_type != DM_F32 && d->c_type != DM_BF16 && !fmt_ok(d->c_type)) return DM_ERR_ARG;
     if (d->m == 0) return DM_OK;
     const int kp = mx_padded(d->k);
-    if (const int rc = operand(d->x, d->ldx, d->x_scales, d->ld_xs, kp, d->x_fmt)) return rc;
+    if (d->x_src == DM_X_MX) {
+        if (const int rc = operand(d->x, d->ldx, d->x_scales, d->ld_xs, kp, d->x_fmt)) return rc;
+    } else if (!d->x || d->ldx < d->k || d->m > DM_X_ROWS_MAX_M || (d->x_src != DM_X_BF16 && d->x_src != DM_X_F32)) {
+        return DM_ERR_ARG;
+    }
     if (const int rc = operand(d->w, d->ldw, d->w_scales, d->ld_ws, kp, d->w_fmt)) return rc;
     MxArgs p = {};
-    p.x = d->x; p.xs = d->x_scales; p.w = d->w; p.ws = d->w_scales;
+    p.x = static_cast<const unsigned char*>(d->x); p.xs = d->x_scales; p.w = d->w; p.ws = d->w_scales;
     p.ldx = d->ldx; p.ld_xs = d->ld_xs; p.ldw = d->ldw; p.ld_ws = d->ld_ws;
     p.m = d->m; p.n_out = d->epi == DM_EPI_GEGLU ? d->n / 2 : d->n; p.n_pad = p.n_out;
     p.nkt = kp / MX_PAD;
@@ -388,6 +483,15 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
         if (!d->c || d->ldc < p.n_out || (d->r && d->ldr < p.n_out)) return DM_ERR_ARG;
         p.vec = dm_aligned16(d->c) && (d->ldc * esz) % 16 == 0 && (!d->r || (dm_aligned16(d->r) && (d->ldr * esz) % 16 == 0));
     }
-    if (d->x_fmt == DM_MXFP8) return d->w_fmt == DM_MXFP8 ? launch_type<8, 8>(p, stream) : launch_type<8, 4>(p, stream);
-    return d->w_fmt == DM_MXFP8 ? launch_type<4, 8>(p, stream) : launch_type<4, 4>(p, stream);
+    if (d->x_src != DM_X_MX) {
+        const int esz = d->x_src == DM_X_F32 ? 4 : 2;
+        p.ldx = d->ldx * esz;  // bytes, as for codes
+        p.k = d->k;
+        p.xvec = dm_aligned16(d->x) && p.ldx % 16 == 0;
+    }
+    const bool exact = d->c_type == DM_F32;
+    int fm, fn;
+    if (split_tile(p, &fm, &fn)) return dm_mx_split_launch(p, d->x_fmt, d->w_fmt, exact, d->x_src, fm, fn, stream);
+    if (d->x_fmt == DM_MXFP8) return d->w_fmt == DM_MXFP8 ? launch_tile<8, 8>(p, exact, stream) : launch_tile<8, 4>(p, exact, stream);
+    return d->w_fmt == DM_MXFP8 ? launch_tile<4, 8>(p, exact, stream) : launch_tile<4, 4>(p, exact, stream);
 }

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import MxGemmDesc, RowNormDesc, check
-from .schedulers.base_scheduler import require_hip, stream_of
+from .schedulers.base_scheduler import require_hip
 
 FORMATS = {"mxfp8": _lib.DM_MXFP8, "mxfp4": _lib.DM_MXFP4}
 _DTYPES = {torch.float32: _lib.DM_F32, torch.bfloat16: _lib.DM_BF16}
@@ -49,10 +49,10 @@ class MXTensor:
             raise ValueError(f"MXTensor: k must be between 1 and {MAX_K}, got {k}")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
             raise RuntimeError("MXTensor: codes and scales are 2-D uint8 tensors")
-        rows = codes.shape[0]
-        if codes.shape[1] != kp * bits // 8 or scales.shape != (rows, kp // BLOCK):
+        (rows, width), shape = codes.shape, scales.shape
+        if width != kp * bits // 8 or shape != (rows, kp // BLOCK):
             raise RuntimeError(f"MXTensor: {fmt} rows of {k} values are {kp * bits // 8} code and {kp // BLOCK} scale bytes, got "
-                               f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+                               f"{tuple(codes.shape)} and {tuple(shape)}")
         if codes.device != scales.device:
             raise RuntimeError(f"MXTensor: codes are on {codes.device}, scales on {scales.device}")
         self.codes, self.scales, self.k, self.fmt = codes, scales, k, fmt
@@ -88,9 +88,9 @@ def _new(rows: int, k: int, fmt: str, device) -> MXTensor:
     return t
 
 
-def _rows(t: torch.Tensor, what: str, name: str) -> torch.Tensor:
-    """``t`` as the kernels read it: 2-D rows on the device, values next to each other (a single row may have any stride)."""
-    if t.device.type != "cuda":
+def _rows(t: torch.Tensor, what: str, name: str) -> None:
+    """Refuses what the kernels do not read: they take 2-D rows on the device, a row's values next to each other."""
+    if not t.is_cuda:
         require_hip(t, what)
     if t.dim() != 2:
         raise RuntimeError(f"{what}: {name} must be a 2-D matrix of rows, got {tuple(t.shape)}")
@@ -98,12 +98,11 @@ def _rows(t: torch.Tensor, what: str, name: str) -> torch.Tensor:
         raise RuntimeError(f"{what}: {name} has dtype {t.dtype}; float32 or bfloat16 are supported")
     if t.shape[1] > 1 and t.stride(1) != 1:
         raise RuntimeError(f"{what}: the values of a row of {name} must be next to each other (stride {t.stride()})")
-    return t
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Row stride; torch gives a single row any stride, and an expanded one 0."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+def _ld(t: torch.Tensor, rows: int, k: int) -> int:
+    """Row stride in elements; torch gives a single row any stride."""
+    return k if rows <= 1 else t.stride(0)
 
 
 def _vector(t: Optional[torch.Tensor], n: int, device, what: str, name: str) -> Optional[int]:
@@ -119,21 +118,21 @@ def _check_width(k: int, what: str):
         raise ValueError(f"{what}: rows must have between 1 and {MAX_K} values, got {k}")
 
 
-class _On:
-    """Kernel launches go to the current device: make it the operands' one for the call."""
-    __slots__ = ("index", "before")
+# The raw stream handle without a Stream object around it: a call here takes 6 to 9 us on the host, of which that was 2.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
-    def __init__(self, device):
-        self.index = device.index
 
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _call(fn, what: str, device: torch.device, *args):
+    """One C entry point on the current stream of ``device``.  Launches go to the current device: make it that one meanwhile."""
+    index = device.index
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MXTensor:
@@ -142,20 +141,25 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MXTensor:
     _rows(x, "mx.quantize", "x")
     rows, k = x.shape
     _check_width(k, "mx.quantize")
-    out = _new(rows, k, fmt, x.device)
-    with _On(x.device):
-        check(_lib.lib().dm_mx_quantize(x.data_ptr(), _ld(x), rows, k, _DTYPES[x.dtype], bits, out.codes.data_ptr(), out.codes.shape[1],
-                                        out.scales.data_ptr(), out.scales.shape[1], stream_of(x)), "mx_quantize")
+    device = x.device
+    out = _new(rows, k, fmt, device)
+    kp = _padded(k)
+    _call(_lib.lib().dm_mx_quantize, "mx_quantize", device, x.data_ptr(), _ld(x, rows, k), rows, k, _DTYPES[x.dtype], bits,
+          out.codes.data_ptr(), kp * bits // 8, out.scales.data_ptr(), kp // BLOCK)
     return out
 
 
 def _operand(t: MXTensor, what: str):
     """(codes, row bytes, scales, row bytes) for the C entry points."""
-    if t.codes.device.type != "cuda":
-        require_hip(t.codes, what)
-    if t.codes.stride(1) != 1 or (t.scales.shape[1] > 1 and t.scales.stride(1) != 1):
+    codes, scales = t.codes, t.scales
+    if not codes.is_cuda:
+        require_hip(codes, what)
+    (ldc, one), (lds, also) = codes.stride(), scales.stride()
+    if one != 1 or also != 1:
         raise RuntimeError(f"{what}: the bytes of a row of an MXTensor must be next to each other")
-    return t.codes.data_ptr(), _ld(t.codes), t.scales.data_ptr(), _ld(t.scales)
+    if codes.shape[0] <= 1:
+        ldc, lds = codes.shape[1], scales.shape[1]
+    return codes.data_ptr(), ldc, scales.data_ptr(), lds
 
 
 def dequantize(t: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -163,10 +167,9 @@ def dequantize(t: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     if dtype not in _DTYPES:
         raise RuntimeError(f"mx.dequantize: dtype {dtype} is not supported (float32 or bfloat16)")
     codes, ldc, scales, lds = _operand(t, "mx.dequantize")
-    out = torch.empty(t.rows, t.k, dtype=dtype, device=t.device)
-    with _On(t.device):
-        check(_lib.lib().dm_mx_dequantize(codes, ldc, scales, lds, t.rows, t.k, FORMATS[t.fmt], out.data_ptr(), t.k, _DTYPES[dtype],
-                                          stream_of(out)), "mx_dequantize")
+    device, rows, k = t.codes.device, t.codes.shape[0], t.k
+    out = torch.empty(rows, k, dtype=dtype, device=device)
+    _call(_lib.lib().dm_mx_dequantize, "mx_dequantize", device, codes, ldc, scales, lds, rows, k, FORMATS[t.fmt], out.data_ptr(), k, _DTYPES[dtype])
     return out
 
 
@@ -174,25 +177,25 @@ def _norm(what, kind, x, weight, bias, residual, eps, out_format):
     _rows(x, what, "x")
     rows, c = x.shape
     _check_width(c, what)
-    d = RowNormDesc(x=x.data_ptr(), ldx=_ld(x), gamma=_vector(weight, c, x.device, what, "weight"), beta=_vector(bias, c, x.device, what, "bias"),
-                    rows=rows, c=c, dtype=_DTYPES[x.dtype], kind=kind, eps=eps)
-    h = None
+    device, dtype = x.device, x.dtype
+    h, r_ptr, ldr, h_ptr = None, None, 0, None
     if residual is not None:
         _rows(residual, what, "residual")
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
-            raise RuntimeError(f"{what}: residual must match x ({x.dtype} {tuple(x.shape)} on {x.device}), got {residual.dtype} "
+        if residual.shape != x.shape or residual.dtype != dtype or residual.device != device:
+            raise RuntimeError(f"{what}: residual must match x ({dtype} {tuple(x.shape)} on {device}), got {residual.dtype} "
                                f"{tuple(residual.shape)} on {residual.device}")
-        h = torch.empty(rows, c, dtype=x.dtype, device=x.device)
-        d.r, d.ldr, d.h, d.ldh = residual.data_ptr(), _ld(residual), h.data_ptr(), c
+        h = torch.empty(rows, c, dtype=dtype, device=device)
+        r_ptr, ldr, h_ptr = residual.data_ptr(), _ld(residual, rows, c), h.data_ptr()
     if out_format is None:
-        y = torch.empty(rows, c, dtype=x.dtype, device=x.device)
-        d.y, d.ldy = y.data_ptr(), c
+        y = torch.empty(rows, c, dtype=dtype, device=device)
+        bits, y_ptr, ldy, ys_ptr, ldys = 0, y.data_ptr(), c, None, 0
     else:
-        d.out_fmt = _format(out_format)
-        y = _new(rows, c, out_format, x.device)
-        d.y, d.ldy, d.y_scales, d.ldys = y.codes.data_ptr(), y.codes.shape[1], y.scales.data_ptr(), y.scales.shape[1]
-    with _On(x.device):
-        check(_lib.lib().dm_row_norm(byref(d), stream_of(x)), "row_norm")
+        bits, kp = _format(out_format), _padded(c)
+        y = _new(rows, c, out_format, device)
+        y_ptr, ldy, ys_ptr, ldys = y.codes.data_ptr(), kp * bits // 8, y.scales.data_ptr(), kp // BLOCK
+    d = RowNormDesc(x.data_ptr(), _ld(x, rows, c), r_ptr, ldr, h_ptr, c, _vector(weight, c, device, what, "weight"),
+                    _vector(bias, c, device, what, "bias"), y_ptr, ldy, ys_ptr, ldys, rows, c, _DTYPES[dtype], kind, bits, eps)
+    _call(_lib.lib().dm_row_norm, "row_norm", device, byref(d))
     return y if h is None else (y, h)
 
 
@@ -224,38 +227,47 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
         raise ValueError(f"{what}: unknown activation {activation!r}")
     if not isinstance(w, MXTensor):
         raise RuntimeError(f"{what}: w must be an MXTensor (mx.quantize)")
+    x_src = _lib.X_MX
     if not isinstance(x, MXTensor):
-        x = quantize(x, x_format)
-    if x.k != w.k:
-        raise RuntimeError(f"{what}: x has rows of {x.k} values, w of {w.k}")
-    if x.device != w.device:
-        raise RuntimeError(f"{what}: x is on {x.device}, w on {w.device}")
-    m, n, device = x.rows, w.rows, x.device
+        bits = _format(x_format)
+        _rows(x, what, "x")
+        if x.shape[0] <= _lib.X_ROWS_MAX_M:
+            # few rows: the product quantises them itself as it reads them (1 x 1280 x 1280: one launch of two)
+            x_src = _lib.X_BF16 if x.dtype == torch.bfloat16 else _lib.X_F32
+            (m, k), device = x.shape, x.device
+            x_ptr, ldx, xs_ptr, ld_xs = x.data_ptr(), _ld(x, m, k), None, 0
+        else:
+            x = quantize(x, x_format)
+    if x_src == _lib.X_MX:
+        bits, m, k, device = FORMATS[x.fmt], x.codes.shape[0], x.k, x.codes.device
+        x_ptr, ldx, xs_ptr, ld_xs = _operand(x, what)
+    if k != w.k:
+        raise RuntimeError(f"{what}: x has rows of {k} values, w of {w.k}")
+    if device != w.codes.device:
+        raise RuntimeError(f"{what}: x is on {device}, w on {w.codes.device}")
+    n = w.codes.shape[0]
     if n < 1 or (activation == "geglu" and n % 2):
         raise RuntimeError(f"{what}: {n} output columns" + (" cannot be halved for geglu" if n else ""))
     wide = n // 2 if activation == "geglu" else n
-    d = MxGemmDesc()
-    d.x, d.ldx, d.x_scales, d.ld_xs = _operand(x, what)
-    d.w, d.ldw, d.w_scales, d.ld_ws = _operand(w, what)
-    d.x_fmt, d.w_fmt, d.m, d.n, d.k, d.epi = FORMATS[x.fmt], FORMATS[w.fmt], m, n, x.k, _ACTIVATIONS[activation]
-    d.bias = _vector(bias, n, device, what, "bias")
+    r_ptr, ldr, cs_ptr, ld_cs = None, 0, None, 0
     if out_format is None:
         if out_dtype not in _DTYPES:
             raise RuntimeError(f"{what}: out_dtype {out_dtype} is not supported (float32 or bfloat16)")
         y = torch.empty(m, wide, dtype=out_dtype, device=device)
-        d.c, d.ldc, d.c_type = y.data_ptr(), wide, _DTYPES[out_dtype]
+        c_ptr, ldc, c_type = y.data_ptr(), wide, _DTYPES[out_dtype]
         if residual is not None:
             _rows(residual, what, "residual")
             if residual.shape != y.shape or residual.dtype != out_dtype or residual.device != device:
                 raise RuntimeError(f"{what}: residual must match the result ({out_dtype} {tuple(y.shape)} on {device}), got "
                                    f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
-            d.r, d.ldr = residual.data_ptr(), _ld(residual)
+            r_ptr, ldr = residual.data_ptr(), _ld(residual, m, wide)
     else:
         if residual is not None:
             raise RuntimeError(f"{what}: a quantised result takes no residual")
-        d.c_type = _format(out_format)
+        c_type, kp = _format(out_format), _padded(wide)
         y = _new(m, wide, out_format, device)
-        d.c, d.ldc, d.c_scales, d.ld_cs = y.codes.data_ptr(), y.codes.shape[1], y.scales.data_ptr(), y.scales.shape[1]
-    with _On(device):
-        check(_lib.lib().dm_mx_gemm(byref(d), torch.cuda.current_stream(device).cuda_stream), "mx_gemm")
+        c_ptr, ldc, cs_ptr, ld_cs = y.codes.data_ptr(), kp * c_type // 8, y.scales.data_ptr(), kp // BLOCK
+    d = MxGemmDesc(x_ptr, ldx, xs_ptr, ld_xs, *_operand(w, what), bits, FORMATS[w.fmt], x_src, m, n, k, _vector(bias, n, device, what, "bias"),
+                   r_ptr, ldr, c_ptr, ldc, cs_ptr, ld_cs, c_type, _ACTIVATIONS[activation])
+    _call(_lib.lib().dm_mx_gemm, "mx_gemm", device, byref(d))
     return y

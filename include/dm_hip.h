@@ -334,18 +334,25 @@ typedef struct DmRowNormDesc {
 int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream);
 
 /* Product of two MX matrices, C = act(X W^T + bias) + r: X m x k, W n x k (both formats, in any combination).
+ * x_src DM_X_MX: X is such a matrix (rows of at most 2^24 bytes, as W's).  DM_X_BF16 / DM_X_F32: x points at plain rows of ldx
+ * elements (any alignment), which are quantised to x_fmt as they are read - the codes that dm_mx_quantize gives, without its
+ * launch; for at most DM_X_ROWS_MAX_M rows, x_scales unused.
  * epi: DM_EPI_PLAIN, DM_EPI_QUICKGELU, or DM_EPI_GEGLU (rows 0 .. n/2 of W are the values, the others the gates; n even; C has
  * n/2 columns).  bias: n fp32 or NULL.  c_type: DM_BF16 / DM_F32 (rows of ldc elements; r, optional, has the same type), or
  * DM_MXFP8 / DM_MXFP4 (c = codes, ldc bytes; c_scales, ld_cs; no r): an MX matrix ready to be the next product's X.
  * Accumulation in fp32.  DM_BF16 and MX results come from the scaled matrix instructions on the codes themselves, whose adder
  * drops low bits of e4m3 products (2e-5 of the result on normal data); DM_F32 results with an e4m3 operand from bf16 matrix instructions on
  * the decoded operands, which are exact there. */
+#define DM_X_MX 0
+#define DM_X_BF16 1
+#define DM_X_F32 2
+#define DM_X_ROWS_MAX_M 16
 typedef struct DmMxGemmDesc {
-    const unsigned char* x; long ldx;
+    const void* x; long ldx;
     const unsigned char* x_scales; long ld_xs;
     const unsigned char* w; long ldw;
     const unsigned char* w_scales; long ld_ws;
-    int x_fmt, w_fmt;
+    int x_fmt, w_fmt, x_src;
     int m, n, k;
     const float* bias;
     const void* r; long ldr;

@@ -530,3 +530,22 @@ def test_feed_forward_on_another_stream_and_in_a_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, feed_forward(x.clone(), *args[1:]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
+@pytest.mark.parametrize("m,n,k", [(4000, 3700, 160), (2050, 4200, 1400), (1100, 9000, 40)])
+@pytest.mark.parametrize("activation,out", [(None, torch.bfloat16), ("geglu", "mxfp8"), ("quick_gelu", torch.float32)], ids=["bf16", "geglu-mx8", "gelu-f32"])
+def test_linear_tiles_of_large_products(dev, xf, wf, m, n, k, activation, out):
+    """Sizes at which the large tiles are taken, with ragged edges on all sides; 64-bit reference on the device."""
+    gen = torch.Generator(device=dev).manual_seed(m)
+    x = mx.quantize(torch.randn(m, k, generator=gen, device=dev), xf)
+    w = mx.quantize(torch.randn(n, k, generator=gen, device=dev) / math.sqrt(k), wf)
+    b = torch.randn(n, generator=gen, device=dev)
+    res = torch.randn(m, n, generator=gen, device=dev).to(out) if out == torch.bfloat16 else None
+    got = mx.linear(x, w, b, activation=activation, **(dict(out_format=out) if isinstance(out, str) else dict(out_dtype=out, residual=res)))
+    got = mx.dequantize(got) if isinstance(out, str) else got
+    xv, wv = mx.dequantize(x).double(), mx.dequantize(w).double()
+    y = torch.mm(xv, wv.t().contiguous()) + b.double()
+    size = torch.mm(xv.abs(), wv.abs().t().contiguous()) + b.double().abs()
+    check_linear(y, size, k, got, activation, out, res, (xf, wf) != ("mxfp4", "mxfp4") and out != torch.float32)
