@@ -1,5 +1,5 @@
 // Quantisation to the microscaled (MX) formats and back, and the row norms (RMS / layer norm with the residual's addition)
-// that write them.  All of it is bound by HBM: every value is read once, with 16-byte accesses where rows are aligned.
+// that write them.  All of it is bound by HBM: every value is read once, with 16-byte accesses whatever the rows' alignment.
 #include "dm_hip.h"
 #include "mx.h"
 
@@ -8,23 +8,21 @@ namespace {
 constexpr int THREADS = 256;
 
 // Eight consecutive values at p, of which those below `left` exist (the others read as zero).
-template <typename T> __device__ __forceinline__ void load8(const T* p, int left, bool vec, float* v) {
+template <typename T> __device__ __forceinline__ void load8(const T* p, int left, float* v) {
     constexpr int EPC = ElemTraits<T>::EPC;
-    if (vec) {  // left is 8 or more, or nothing exists
+    if (left >= 8) {
 #pragma unroll
-        for (int c = 0; c < 8 / EPC; ++c) chunk_to_f32<T>(ldg16(p + c * EPC, left >= 8), v + c * EPC);
+        for (int c = 0; c < 8 / EPC; ++c) chunk_to_f32<T>(load16_any(p + c * EPC), v + c * EPC);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < left ? ElemTraits<T>::load(p + i) : 0.f;
     }
 }
-template <typename T> __device__ __forceinline__ void store8(T* p, int left, bool vec, const float* v) {
+template <typename T> __device__ __forceinline__ void store8(T* p, int left, const float* v) {
     constexpr int EPC = ElemTraits<T>::EPC;
-    if (vec) {
-        if (left >= 8) {
+    if (left >= 8) {
 #pragma unroll
-            for (int c = 0; c < 8 / EPC; ++c) *reinterpret_cast<u32x4*>(p + c * EPC) = f32_to_chunk<T>(v + c * EPC);
-        }
+        for (int c = 0; c < 8 / EPC; ++c) store16_any(p + c * EPC, f32_to_chunk<T>(v + c * EPC));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -35,49 +33,68 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int left, boo
 // ---- quantise / dequantise ------------------------------------------------------------------------------------------
 // A lane holds eight values, a quad the 32 of a block.  `gpr` = groups of eight per padded row (a multiple of 16), so a
 // quad never straddles rows; a block sweeps UNROLL x 256 consecutive groups with all its loads ahead of the arithmetic.
-constexpr int UNROLL = 4;
+struct Groups {
+    int gpr;
+    uint32_t magic;  // ceil(2^32 / gpr)
+    double inverse;  // 1 / gpr
+    long total;
+    // group `first` as (row, group of the row); the estimate is off by one row at most
+    __device__ __forceinline__ void split(long first, long& row, int& g) const {
+        row = (long)((double)first * inverse);
+        long rest = first - row * gpr;
+        if (rest < 0) { --row; rest += gpr; }
+        if (rest >= gpr) { ++row; rest -= gpr; }
+        g = (int)rest;
+    }
+    // at / gpr for at < gpr + 1024 * UNROLL: multiplied while at * gpr < 2^32 makes that exact
+    __device__ __forceinline__ uint32_t rows_in(uint32_t at) const {
+        return gpr < 16384 ? __umulhi(at, magic) : (at >= (uint32_t)gpr);
+    }
+};
 
-template <typename T, int FMT>
-__global__ __launch_bounds__(THREADS) void mx_quantize_kernel(const T* __restrict__ x, long ldx, long total, int gpr, int k, bool vec,
+template <typename T, int FMT, int UNROLL>
+__global__ __launch_bounds__(THREADS) void mx_quantize_kernel(const T* __restrict__ x, long ldx, Groups n, int k,
                                                                unsigned char* __restrict__ codes, long ldc,
                                                                unsigned char* __restrict__ scales, long lds) {
     const long first = (long)blockIdx.x * (THREADS * UNROLL);
-    const long row0 = first / gpr;
-    const int g0 = (int)(first - row0 * gpr);
+    long row0;
+    int g0;
+    n.split(first, row0, g0);
     float v[UNROLL][8];
     long row[UNROLL];
     int g[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const unsigned at = g0 + u * THREADS + threadIdx.x;
-        const unsigned r = at / (unsigned)gpr;
+        const unsigned r = n.rows_in(at);
         row[u] = row0 + r;
-        g[u] = at - r * gpr;
-        if (first + u * THREADS + threadIdx.x < total) load8<T>(x + row[u] * ldx + g[u] * 8, k - g[u] * 8, vec, v[u]);
+        g[u] = at - r * n.gpr;
+        if (first + u * THREADS + threadIdx.x < n.total) load8<T>(x + row[u] * ldx + g[u] * 8, k - g[u] * 8, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-        if (first + u * THREADS + threadIdx.x < total)
+        if (first + u * THREADS + threadIdx.x < n.total)
             mx_store_quad<FMT>(v[u], codes + row[u] * ldc + g[u] * mx_bytes(FMT, 8), scales + row[u] * lds + (g[u] >> 2), threadIdx.x);
 }
 
-template <typename T, int FMT>
+template <typename T, int FMT, int UNROLL>
 __global__ __launch_bounds__(THREADS) void mx_dequantize_kernel(const unsigned char* __restrict__ codes, long ldc,
-                                                                 const unsigned char* __restrict__ scales, long lds, long total, int gpr,
-                                                                 int k, bool vec, T* __restrict__ y, long ldy) {
+                                                                 const unsigned char* __restrict__ scales, long lds, Groups n,
+                                                                 int k, T* __restrict__ y, long ldy) {
     const long first = (long)blockIdx.x * (THREADS * UNROLL);
-    const long row0 = first / gpr;
-    const int g0 = (int)(first - row0 * gpr);
+    long row0;
+    int g0;
+    n.split(first, row0, g0);
     uint32_t w[UNROLL][2], s[UNROLL];
     long row[UNROLL];
     int g[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const unsigned at = g0 + u * THREADS + threadIdx.x;
-        const unsigned r = at / (unsigned)gpr;
+        const unsigned r = n.rows_in(at);
         row[u] = row0 + r;
-        g[u] = at - r * gpr;
-        if (first + u * THREADS + threadIdx.x < total) {
+        g[u] = at - r * n.gpr;
+        if (first + u * THREADS + threadIdx.x < n.total) {
             const uint32_t* p = reinterpret_cast<const uint32_t*>(codes + row[u] * ldc + g[u] * mx_bytes(FMT, 8));
             if constexpr (FMT == 8) {
                 const u32x2 t = *reinterpret_cast<const u32x2*>(p);
@@ -91,10 +108,10 @@ __global__ __launch_bounds__(THREADS) void mx_dequantize_kernel(const unsigned c
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-        if (first + u * THREADS + threadIdx.x < total) {
+        if (first + u * THREADS + threadIdx.x < n.total) {
             float v[8];
             mx_decode8<FMT>(w[u], mx_scale(s[u]), v);
-            store8<T>(y + row[u] * ldy + g[u] * 8, k - g[u] * 8, vec, v);
+            store8<T>(y + row[u] * ldy + g[u] * 8, k - g[u] * 8, v);
         }
 }
 
@@ -111,13 +128,20 @@ struct NormArgs {
     long rows;
     int c, layer;
     float eps;
-    bool vec;
 };
 
-// Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.
+// Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.  Inside 16 lanes by DPP (a shuffle
+// through LDS takes an order of magnitude longer, and short rows are bound by this chain).
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    v = dpp_add<0xB1>(v);   // quad_perm 1 0 3 2
+    v = dpp_add<0x4E>(v);   // quad_perm 2 3 0 1
+    v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of eight lanes
+    v = dpp_add<0x140>(v);  // row_mirror: the other eight of sixteen
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
     if constexpr (TPR > 64) {
         __syncthreads();  // the previous sum has been read
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -130,10 +154,10 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red)
 }
 // eight values of h = x + r, rounded to the storage type (the norm is that of the stored row)
 template <typename T> __device__ __forceinline__ void load_h(const NormArgs& p, long row, int at, float* v) {
-    load8<T>(static_cast<const T*>(p.x) + row * p.ldx + at, p.c - at, p.vec, v);
+    load8<T>(static_cast<const T*>(p.x) + row * p.ldx + at, p.c - at, v);
     if (p.r) {
         float r[8];
-        load8<T>(static_cast<const T*>(p.r) + row * p.ldr + at, p.c - at, p.vec, r);
+        load8<T>(static_cast<const T*>(p.r) + row * p.ldr + at, p.c - at, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[i] += r[i];
@@ -141,18 +165,21 @@ template <typename T> __device__ __forceinline__ void load_h(const NormArgs& p, 
         }
     }
 }
-template <typename T, int OUT> __device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, float rstd) {
-    float w[8], o[8];
-    load8<float>(p.gamma + at, p.c - at, p.vec, w);
+__device__ __forceinline__ void load_affine(const NormArgs& p, int at, float* gamma, float* beta) {
+    load8<float>(p.gamma + at, p.c - at, gamma);
+    if (p.beta) load8<float>(p.beta + at, p.c - at, beta);
+}
+template <typename T, int OUT>
+__device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, float rstd, const float* gamma, const float* beta) {
+    float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (v[i] - mean) * rstd * w[i];
+    for (int i = 0; i < 8; ++i) o[i] = (v[i] - mean) * rstd * gamma[i];
     if (p.beta) {
-        load8<float>(p.beta + at, p.c - at, p.vec, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] += w[i];
+        for (int i = 0; i < 8; ++i) o[i] += beta[i];
     }
     if constexpr (OUT == 0) {
-        store8<T>(static_cast<T*>(p.y) + row * p.ldy + at, p.c - at, p.vec, o);
+        store8<T>(static_cast<T*>(p.y) + row * p.ldy + at, p.c - at, o);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = at + i < p.c ? o[i] : 0.f;
@@ -172,11 +199,18 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
     float v[NV][8];
 #pragma unroll
     for (int n = 0; n < NV; ++n) load_h<T>(p, row, (n * TPR + t) * 8, v[n]);
+    // short rows: the scale is on its way while the row is summed; long ones have other rows to wait with
+    constexpr bool EARLY = NV <= 2;
+    float gamma[EARLY ? NV : 1][8], beta[EARLY ? NV : 1][8];
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) load_affine(p, (n * TPR + t) * 8, gamma[n], beta[n]);
+    }
     float s = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
         const int at = (n * TPR + t) * 8;
-        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, p.vec, v[n]);
+        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, v[n]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += p.layer ? v[n][i] : v[n][i] * v[n][i];
     }
@@ -197,7 +231,10 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
     const float rstd = 1.f / sqrtf(s + p.eps);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
-        if ((n * TPR + t) * 8 < cp) norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, rstd);
+        if ((n * TPR + t) * 8 < cp) {
+            if constexpr (!EARLY) load_affine(p, (n * TPR + t) * 8, gamma[0], beta[0]);
+            norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, rstd, gamma[EARLY ? n : 0], beta[EARLY ? n : 0]);
+        }
 }
 
 // Rows too long for registers: one block per row sweeps it once per sum and once for the output; the sweeps behind the
@@ -212,7 +249,7 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
     for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
         float v[8];
         load_h<T>(p, row, at, v);
-        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, p.vec, v);
+        if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += p.layer ? v[i] : v[i] * v[i];
     }
@@ -222,7 +259,7 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
         s = 0.f;
         for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
             float v[8];
-            load8<T>(stored + at, p.c - at, p.vec, v);
+            load8<T>(stored + at, p.c - at, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = at + i < p.c ? v[i] - mean : 0.f;
@@ -234,8 +271,10 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
     const float rstd = 1.f / sqrtf(s + p.eps);
     for (int at = threadIdx.x * 8; at < cp; at += THREADS * 8) {
         float v[8];
-        load8<T>(stored + at, p.c - at, p.vec, v);
-        norm_store<T, OUT>(p, row, at, v, mean, rstd);
+        load8<T>(stored + at, p.c - at, v);
+        float gamma[8], beta[8];
+        load_affine(p, at, gamma, beta);
+        norm_store<T, OUT>(p, row, at, v, mean, rstd, gamma, beta);
     }
 }
 
@@ -256,8 +295,6 @@ template <typename T, int OUT> int launch_norm(const NormArgs& p, hipStream_t s)
 
 bool mx_fmt_ok(int fmt) { return fmt == DM_MXFP8 || fmt == DM_MXFP4; }
 bool dtype_ok(int dtype) { return dtype == DM_F32 || dtype == DM_BF16; }
-int esize(int dtype) { return dtype == DM_F32 ? 4 : 2; }
-bool rows_vec(const void* p, long ld, int esz) { return dm_aligned16(p) && (ld * esz) % 16 == 0; }
 // codes / scales of `rows` rows of k values: 0 or an error code
 int mx_layout(const void* codes, long ldc, const void* scales, long lds, int k, int fmt) {
     if (!codes || !scales || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
@@ -268,6 +305,16 @@ int mx_layout(const void* codes, long ldc, const void* scales, long lds, int k, 
 }
 constexpr int MAX_K = 1 << 24;       // values of a row: 32-bit offsets inside a row
 constexpr long MAX_GRID = 0x7fffffffL;
+Groups groups_of(long rows, int k) {
+    Groups n;
+    n.gpr = mx_padded(k) / 8;
+    n.magic = (uint32_t)((0x100000000ULL + n.gpr - 1) / n.gpr);
+    n.inverse = 1.0 / n.gpr;
+    n.total = rows * n.gpr;
+    return n;
+}
+// Four groups per thread once that leaves eight blocks per CU; fewer values are spread over more CUs.
+int unroll_of(long total) { return total >= 2048L * THREADS * 4 ? 4 : 1; }
 
 }  // namespace
 
@@ -277,13 +324,13 @@ extern "C" int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dty
     if (rows == 0) return DM_OK;
     if (!x || ldx < k) return DM_ERR_ARG;
     if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
-    const int gpr = mx_padded(k) / 8;
-    const long total = rows * gpr, blocks = (total + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks > MAX_GRID) return DM_ERR_ARG;
-    const bool vec = k % 8 == 0 && rows_vec(x, ldx, esize(dtype));
-    const dim3 grid((unsigned)blocks);
-#define DM_MX_Q(T, F) \
-    mx_quantize_kernel<T, F><<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), ldx, total, gpr, k, vec, codes, ldc, scales, lds)
+    const Groups n = groups_of(rows, k);
+    if (n.total > MAX_GRID * THREADS) return DM_ERR_ARG;
+    const int unroll = unroll_of(n.total);
+    const dim3 grid((unsigned)((n.total + THREADS * unroll - 1) / (THREADS * unroll)));
+#define DM_MX_Q(T, F)                                                                                                                   \
+    (unroll == 1 ? mx_quantize_kernel<T, F, 1><<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), ldx, n, k, codes, ldc, scales, lds) \
+                 : mx_quantize_kernel<T, F, 4><<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x), ldx, n, k, codes, ldc, scales, lds))
     if (dtype == DM_F32) { if (fmt == DM_MXFP8) DM_MX_Q(float, 8); else DM_MX_Q(float, 4); }
     else { if (fmt == DM_MXFP8) DM_MX_Q(bf16_t, 8); else DM_MX_Q(bf16_t, 4); }
 #undef DM_MX_Q
@@ -296,13 +343,13 @@ extern "C" int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsi
     if (rows == 0) return DM_OK;
     if (!y || ldy < k) return DM_ERR_ARG;
     if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
-    const int gpr = mx_padded(k) / 8;
-    const long total = rows * gpr, blocks = (total + THREADS * UNROLL - 1) / (THREADS * UNROLL);
-    if (blocks > MAX_GRID) return DM_ERR_ARG;
-    const bool vec = k % 8 == 0 && rows_vec(y, ldy, esize(dtype));
-    const dim3 grid((unsigned)blocks);
-#define DM_MX_D(T, F) \
-    mx_dequantize_kernel<T, F><<<grid, THREADS, 0, stream>>>(codes, ldc, scales, lds, total, gpr, k, vec, static_cast<T*>(y), ldy)
+    const Groups n = groups_of(rows, k);
+    if (n.total > MAX_GRID * THREADS) return DM_ERR_ARG;
+    const int unroll = unroll_of(n.total);
+    const dim3 grid((unsigned)((n.total + THREADS * unroll - 1) / (THREADS * unroll)));
+#define DM_MX_D(T, F)                                                                                                                     \
+    (unroll == 1 ? mx_dequantize_kernel<T, F, 1><<<grid, THREADS, 0, stream>>>(codes, ldc, scales, lds, n, k, static_cast<T*>(y), ldy) \
+                 : mx_dequantize_kernel<T, F, 4><<<grid, THREADS, 0, stream>>>(codes, ldc, scales, lds, n, k, static_cast<T*>(y), ldy))
     if (dtype == DM_F32) { if (fmt == DM_MXFP8) DM_MX_D(float, 8); else DM_MX_D(float, 4); }
     else { if (fmt == DM_MXFP8) DM_MX_D(bf16_t, 8); else DM_MX_D(bf16_t, 4); }
 #undef DM_MX_D
@@ -315,7 +362,6 @@ extern "C" int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream) {
         return DM_ERR_ARG;
     if (d->rows == 0) return DM_OK;
     if (!d->x || !d->gamma || !d->y || (d->r == nullptr) != (d->h == nullptr)) return DM_ERR_ARG;
-    const int esz = esize(d->dtype);
     if (d->ldx < d->c || (d->r && (d->ldr < d->c || d->ldh < d->c)) || d->rows > MAX_GRID) return DM_ERR_ARG;
     if (d->out_fmt) {
         if (const int rc = mx_layout(d->y, d->ldy, d->y_scales, d->ldys, d->c, d->out_fmt)) return rc;
@@ -326,8 +372,6 @@ extern "C" int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream) {
     p.x = d->x; p.r = d->r; p.h = d->h; p.gamma = d->gamma; p.beta = d->beta; p.y = d->y; p.ys = d->y_scales;
     p.ldx = d->ldx; p.ldr = d->ldr; p.ldh = d->ldh; p.ldy = d->ldy; p.ldys = d->ldys;
     p.rows = d->rows; p.c = d->c; p.layer = d->kind == DM_NORM_LAYER; p.eps = d->eps;
-    p.vec = d->c % 8 == 0 && rows_vec(d->x, d->ldx, esz) && (!d->r || (rows_vec(d->r, d->ldr, esz) && rows_vec(d->h, d->ldh, esz))) &&
-            dm_aligned16(d->gamma) && (!d->beta || dm_aligned16(d->beta)) && (d->out_fmt || rows_vec(d->y, d->ldy, esz));
 #define DM_NORM(T) \
     (d->out_fmt == 0 ? launch_norm<T, 0>(p, stream) : d->out_fmt == DM_MXFP8 ? launch_norm<T, 8>(p, stream) : launch_norm<T, 4>(p, stream))
     return d->dtype == DM_F32 ? DM_NORM(float) : DM_NORM(bf16_t);

@@ -97,7 +97,7 @@ __device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float*
     }
     if (m >= p.m || col >= p.n_out) return;
     const int left = p.n_out - col;
-    const bool whole = p.vec && left >= 16;
+    const bool whole = left >= 16;
     if (p.c_type == DM_BF16) {
         bf16_t* dst = static_cast<bf16_t*>(p.c) + m * p.ldc + col;
         const bf16_t* res = static_cast<const bf16_t*>(p.r) + m * p.ldr + col;
@@ -106,11 +106,11 @@ __device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float*
             for (int h = 0; h < 2; ++h) {
                 if (p.r) {
                     float f[8];
-                    chunk_to_f32<bf16_t>(*reinterpret_cast<const u32x4*>(res + 8 * h), f);
+                    chunk_to_f32<bf16_t>(load16_any(res + 8 * h), f);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[8 * h + i] += f[i];
                 }
-                *reinterpret_cast<u32x4*>(dst + 8 * h) = f32_to_chunk<bf16_t>(v + 8 * h);
+                store16_any(dst + 8 * h, f32_to_chunk<bf16_t>(v + 8 * h));
             }
         } else {
 #pragma unroll
@@ -124,8 +124,8 @@ __device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float*
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 f32x4 o = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-                if (p.r) o += *reinterpret_cast<const f32x4*>(res + 4 * h);
-                *reinterpret_cast<f32x4*>(dst + 4 * h) = o;
+                if (p.r) o += __builtin_bit_cast(f32x4, load16_any(res + 4 * h));
+                store16_any(dst + 4 * h, __builtin_bit_cast(u32x4, o));
             }
         } else {
 #pragma unroll
@@ -365,7 +365,7 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
                     for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_erf_f(acc[i][j + 1][e]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_erf_fast_f(acc[i][j + 1][e]);
+                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_poly_f(acc[i][j + 1][e]);
                 }
                 store16(p, m0 + wm * WM + i * 32 + fr, column(j), v, lane, edge);
             }
@@ -479,15 +479,11 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
         p.n_pad = mx_padded(p.n_out);
         if (const int rc = operand(d->c, d->ldc, d->c_scales, d->ld_cs, p.n_pad, d->c_type)) return rc;
     } else {
-        const int esz = d->c_type == DM_F32 ? 4 : 2;
         if (!d->c || d->ldc < p.n_out || (d->r && d->ldr < p.n_out)) return DM_ERR_ARG;
-        p.vec = dm_aligned16(d->c) && (d->ldc * esz) % 16 == 0 && (!d->r || (dm_aligned16(d->r) && (d->ldr * esz) % 16 == 0));
     }
     if (d->x_src != DM_X_MX) {
-        const int esz = d->x_src == DM_X_F32 ? 4 : 2;
-        p.ldx = d->ldx * esz;  // bytes, as for codes
+        p.ldx = d->ldx * (d->x_src == DM_X_F32 ? 4 : 2);  // bytes, as for codes
         p.k = d->k;
-        p.xvec = dm_aligned16(d->x) && p.ldx % 16 == 0;
     }
     const bool exact = d->c_type == DM_F32;
     int fm, fn;

@@ -4,7 +4,8 @@
 namespace {
 
 // ---- split kernel ----------------------------------------------------------------------------------------------------
-// Few output tiles: the eight waves of a block share one tile of 16 FM rows by 16 FN rows of W and divide its k axis.  Nothing is
+// Few output tiles: the eight waves of a block share one tile of 16 FM rows by 16 FN rows of W; every eighth k-tile is a wave's, so
+// that their reads of a row lie side by side.  Nothing is
 // shared before the end, so operands go from memory straight to registers, UNIT k-tiles at once and without a barrier, and the
 // eight partial sums meet in LDS in a fixed order.  What bounds it is how many cache lines the loads touch, so it uses the
 // 16-row instruction: four lanes read 64 bytes of a row where the 32-row one's two lanes read 32, and the scales of four
@@ -14,11 +15,11 @@ namespace {
 constexpr int SPLIT_WAVES = 8;
 
 // N values from p on, those at `left` and behind as zeros
-template <typename T, int N> __device__ __forceinline__ void load_values(const T* p, int left, bool vec, float* v) {
+template <typename T, int N> __device__ __forceinline__ void load_values(const T* p, int left, float* v) {
     constexpr int EPC = ElemTraits<T>::EPC;
-    if (vec && left >= N) {
+    if (left >= N) {
 #pragma unroll
-        for (int c = 0; c < N / EPC; ++c) chunk_to_f32<T>(*reinterpret_cast<const u32x4*>(p + c * EPC), v + c * EPC);
+        for (int c = 0; c < N / EPC; ++c) chunk_to_f32<T>(load16_any(p + c * EPC), v + c * EPC);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = i < left ? ElemTraits<T>::load(p + i) : 0.f;
@@ -36,7 +37,7 @@ template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::
     }
 }
 template <int F, bool EXACT, typename T>
-__device__ __forceinline__ typename MxFragment<F>::type quantize_fragment16(const T* row, int k, int kt, int lane, bool vec, int& scale) {
+__device__ __forceinline__ typename MxFragment<F>::type quantize_fragment16(const T* row, int k, int kt, int lane, int& scale) {
     const int g = lane >> 4;
     typename MxFragment<F>::type out;
     float v[32];
@@ -45,7 +46,7 @@ __device__ __forceinline__ typename MxFragment<F>::type quantize_fragment16(cons
 #pragma unroll
         for (int b = 0; b < 2; ++b) {  // half a block each; the other half is in lane l ^ 16
             const int at = kt * MX_PAD + 64 * b + 16 * g;
-            load_values<T, 16>(row + at, k - at, vec, v + 16 * b);
+            load_values<T, 16>(row + at, k - at, v + 16 * b);
             float top = mx_largest<16>(v + 16 * b);
             top = __builtin_elementwise_maximum(top, __shfl_xor(top, 16));
             byte[b] = mx_scale_byte<8>(top);  // of block 2 b + g / 2
@@ -55,7 +56,7 @@ __device__ __forceinline__ typename MxFragment<F>::type quantize_fragment16(cons
         scale = g < 2 ? lo : hi;
     } else {
         const int at = kt * MX_PAD + 32 * g;
-        load_values<T, 32>(row + at, k - at, vec, v);
+        load_values<T, 32>(row + at, k - at, v);
         byte[0] = byte[1] = mx_scale_byte<F>(mx_largest<32>(v));
         scale = (int)byte[0];
     }
@@ -94,11 +95,11 @@ __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* 
     if (p.c_type == DM_BF16) {
         bf16_t* dst = static_cast<bf16_t*>(p.c) + m * p.ldc + col;
         float r[8] = {};
-        if (p.r) load_values<bf16_t, 8>(static_cast<const bf16_t*>(p.r) + m * p.ldr + col, left, p.vec, r);
+        if (p.r) load_values<bf16_t, 8>(static_cast<const bf16_t*>(p.r) + m * p.ldr + col, left, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += r[e];
-        if (p.vec && left >= 8) {
-            *reinterpret_cast<u32x4*>(dst) = f32_to_chunk<bf16_t>(v);
+        if (left >= 8) {
+            store16_any(dst, f32_to_chunk<bf16_t>(v));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -107,12 +108,12 @@ __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* 
     } else {
         float* dst = static_cast<float*>(p.c) + m * p.ldc + col;
         float r[8] = {};
-        if (p.r) load_values<float, 8>(static_cast<const float*>(p.r) + m * p.ldr + col, left, p.vec, r);
+        if (p.r) load_values<float, 8>(static_cast<const float*>(p.r) + m * p.ldr + col, left, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += r[e];
-        if (p.vec && left >= 8) {
-            *reinterpret_cast<u32x4*>(dst) = f32_to_chunk<float>(v);
-            *reinterpret_cast<u32x4*>(dst + 4) = f32_to_chunk<float>(v + 4);
+        if (left >= 8) {
+            store16_any(dst, f32_to_chunk<float>(v));
+            store16_any(dst + 4, f32_to_chunk<float>(v + 4));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -152,12 +153,12 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{};
 
     auto process = [&](int kt, auto count) {
-        constexpr int N = decltype(count)::value;  // k-tiles kt .. kt + N - 1
+        constexpr int N = decltype(count)::value;  // k-tiles kt, kt + 8, .. of this wave
         typename MxFragment<XF>::type x[N][FM];
         typename MxFragment<WF>::type w[N][FN];
         int sx[N][FM], sw[N][FN], sxw[FM], sww[FN];
         // lane g: the four scale bytes of k-tile g (mod N) of its row
-        const long sat = 4L * (kt + g % N);
+        const long sat = 4L * (kt + SPLIT_WAVES * (g % N));
 #pragma unroll
         for (int j = 0; j < FN; ++j) sww[j] = *reinterpret_cast<const int*>(wsrow[j] + sat);
 #pragma unroll
@@ -166,12 +167,12 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
 #pragma unroll
-            for (int j = 0; j < FN; ++j) w[u][j] = load_fragment16<WF, EXACT>(wrow[j] + (long)(kt + u) * mx_bytes(WF, MX_PAD), g);
+            for (int j = 0; j < FN; ++j) w[u][j] = load_fragment16<WF, EXACT>(wrow[j] + (long)(kt + SPLIT_WAVES * u) * mx_bytes(WF, MX_PAD), g);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                if constexpr (XSRC == 0) x[u][i] = load_fragment16<XF, EXACT>(xrow[i] + (long)(kt + u) * mx_bytes(XF, MX_PAD), g);
-                if constexpr (XSRC == 1) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const bf16_t*>(xrow[i]), p.k, kt + u, lane, p.xvec, sx[u][i]);
-                if constexpr (XSRC == 2) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const float*>(xrow[i]), p.k, kt + u, lane, p.xvec, sx[u][i]);
+                if constexpr (XSRC == 0) x[u][i] = load_fragment16<XF, EXACT>(xrow[i] + (long)(kt + SPLIT_WAVES * u) * mx_bytes(XF, MX_PAD), g);
+                if constexpr (XSRC == 1) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const bf16_t*>(xrow[i]), p.k, kt + SPLIT_WAVES * u, lane, sx[u][i]);
+                if constexpr (XSRC == 2) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const float*>(xrow[i]), p.k, kt + SPLIT_WAVES * u, lane, sx[u][i]);
             }
         }
 #pragma unroll
@@ -189,13 +190,14 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j) mma16<XF, WF, EXACT>(acc[i][j], x[u][i], w[u][j], sx[u][i], sw[u][j]);
     };
-    for (int kt = wave * UNIT; kt < p.nkt; kt += SPLIT_WAVES * UNIT) {
-        if (kt + UNIT <= p.nkt) {
-            process(kt, std::integral_constant<int, UNIT>());
-        } else {
-            for (int e = kt; e < p.nkt; ++e) process(e, std::integral_constant<int, 1>());
+    int kt = wave;
+    for (; kt + SPLIT_WAVES * (UNIT - 1) < p.nkt; kt += SPLIT_WAVES * UNIT) process(kt, std::integral_constant<int, UNIT>());
+    if constexpr (UNIT == 4)
+        if (kt + SPLIT_WAVES < p.nkt) {
+            process(kt, std::integral_constant<int, 2>());
+            kt += 2 * SPLIT_WAVES;
         }
-    }
+    if (kt < p.nkt) process(kt, std::integral_constant<int, 1>());
 
     // ---- partial sums [wave][fragment][lane]; lane (q, m) of a fragment holds columns 4 q .. 4 q + 3 of row m.  A thread then
     // sums eight columns of one row: four threads to 32 columns.
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
         float gate[8];
         total(2 * (c8 >> 1) + 1, p.n_out + col, gate);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= p.c_type == DM_F32 ? gelu_erf_f(gate[e]) : gelu_erf_fast_f(gate[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= p.c_type == DM_F32 ? gelu_erf_f(gate[e]) : gelu_poly_f(gate[e]);
     } else if (p.epi == DM_EPI_QUICKGELU) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + __expf(-1.702f * v[e]));

@@ -40,7 +40,9 @@ class MXTensor:
     ``codes``: uint8 ``[rows, kp]`` (mxfp8) or ``[rows, kp / 2]`` (mxfp4; the even value in the low nibble) with kp = k rounded
     up to 128 and zeros behind column k; ``scales``: uint8 ``[rows, kp / 32]``.  Both may have a row stride (a multiple of 16 and
     of 4 bytes).  Matrices quantised elsewhere in this format are wrapped as they are."""
-    __slots__ = ("codes", "scales", "k", "fmt")
+    # Results of this module hold one buffer, codes then scales, and make the two views when somebody asks for them: an
+    # allocation or a view costs a small call more than a microsecond each.
+    __slots__ = ("_buffer", "_codes", "_scales", "rows", "k", "fmt", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int, fmt: str):
         bits = _format(fmt)
@@ -55,37 +57,67 @@ class MXTensor:
                                f"{tuple(codes.shape)} and {tuple(shape)}")
         if codes.device != scales.device:
             raise RuntimeError(f"MXTensor: codes are on {codes.device}, scales on {scales.device}")
-        self.codes, self.scales, self.k, self.fmt = codes, scales, k, fmt
+        self._buffer, self._codes, self._scales = None, codes, scales
+        self.rows, self.k, self.fmt, self.device = rows, k, fmt, codes.device
+
+    @classmethod
+    def _empty(cls, rows: int, k: int, fmt: str, bits: int, device):
+        """A new matrix and the four layout arguments of the C entry points: codes, bytes per row, scales, bytes per row."""
+        kp = _padded(k)
+        width, blocks = kp * bits // 8, kp // BLOCK
+        t = cls.__new__(cls)
+        t._buffer = torch.empty(rows * (width + blocks), dtype=torch.uint8, device=device)
+        t._codes = t._scales = None
+        t.rows, t.k, t.fmt, t.device = rows, k, fmt, device
+        at = t._buffer.data_ptr()
+        return t, at, width, at + rows * width, blocks
+
+    def _layout(self, what: str):
+        """The same four arguments of a matrix that is read."""
+        buffer = self._buffer
+        if buffer is not None:
+            kp = _padded(self.k)
+            width, at = kp * FORMATS[self.fmt] // 8, buffer.data_ptr()
+            return at, width, at + self.rows * width, kp // BLOCK
+        codes, scales = self._codes, self._scales
+        if not codes.is_cuda:
+            require_hip(codes, what)
+        (ldc, one), (lds, also) = codes.stride(), scales.stride()
+        if one != 1 or also != 1:
+            raise RuntimeError(f"{what}: the bytes of a row of an MXTensor must be next to each other")
+        if self.rows <= 1:  # torch gives a single row any stride
+            ldc, lds = codes.shape[1], scales.shape[1]
+        return codes.data_ptr(), ldc, scales.data_ptr(), lds
+
+    def _view(self):
+        n = self.rows * (_padded(self.k) * FORMATS[self.fmt] // 8)
+        self._codes = self._buffer[:n].view(self.rows, _padded(self.k) * FORMATS[self.fmt] // 8)
+        self._scales = self._buffer[n:].view(self.rows, _padded(self.k) // BLOCK)
 
     @property
-    def rows(self) -> int:
-        return self.codes.shape[0]
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._view()
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._view()
+        return self._scales
 
     @property
     def shape(self):
-        return (self.codes.shape[0], self.k)
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+        return (self.rows, self.k)
 
     def __repr__(self) -> str:
-        return f"MXTensor({self.rows} x {self.k}, {self.fmt}, {self.codes.device})"
+        return f"MXTensor({self.rows} x {self.k}, {self.fmt}, {self.device})"
 
 
 def _format(fmt: str) -> int:
     if fmt not in FORMATS:
         raise ValueError(f"unknown MX format {fmt!r}; expected one of {sorted(FORMATS)}")
     return FORMATS[fmt]
-
-
-def _new(rows: int, k: int, fmt: str, device) -> MXTensor:
-    kp = _padded(k)
-    t = MXTensor.__new__(MXTensor)
-    t.codes = torch.empty(rows, kp * FORMATS[fmt] // 8, dtype=torch.uint8, device=device)
-    t.scales = torch.empty(rows, kp // BLOCK, dtype=torch.uint8, device=device)
-    t.k, t.fmt = k, fmt
-    return t
 
 
 def _rows(t: torch.Tensor, what: str, name: str) -> None:
@@ -118,7 +150,7 @@ def _check_width(k: int, what: str):
         raise ValueError(f"{what}: rows must have between 1 and {MAX_K} values, got {k}")
 
 
-# The raw stream handle without a Stream object around it: a call here takes 6 to 9 us on the host, of which that was 2.
+# The raw stream handle without a Stream object around it: a call here takes 5 to 9 us on the host, of which that was 2.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
@@ -142,34 +174,19 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MXTensor:
     rows, k = x.shape
     _check_width(k, "mx.quantize")
     device = x.device
-    out = _new(rows, k, fmt, device)
-    kp = _padded(k)
-    _call(_lib.lib().dm_mx_quantize, "mx_quantize", device, x.data_ptr(), _ld(x, rows, k), rows, k, _DTYPES[x.dtype], bits,
-          out.codes.data_ptr(), kp * bits // 8, out.scales.data_ptr(), kp // BLOCK)
+    out, *layout = MXTensor._empty(rows, k, fmt, bits, device)
+    _call(_lib.lib().dm_mx_quantize, "mx_quantize", device, x.data_ptr(), _ld(x, rows, k), rows, k, _DTYPES[x.dtype], bits, *layout)
     return out
-
-
-def _operand(t: MXTensor, what: str):
-    """(codes, row bytes, scales, row bytes) for the C entry points."""
-    codes, scales = t.codes, t.scales
-    if not codes.is_cuda:
-        require_hip(codes, what)
-    (ldc, one), (lds, also) = codes.stride(), scales.stride()
-    if one != 1 or also != 1:
-        raise RuntimeError(f"{what}: the bytes of a row of an MXTensor must be next to each other")
-    if codes.shape[0] <= 1:
-        ldc, lds = codes.shape[1], scales.shape[1]
-    return codes.data_ptr(), ldc, scales.data_ptr(), lds
 
 
 def dequantize(t: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``t`` stands for, ``[rows, k]`` fp32 or bf16."""
     if dtype not in _DTYPES:
         raise RuntimeError(f"mx.dequantize: dtype {dtype} is not supported (float32 or bfloat16)")
-    codes, ldc, scales, lds = _operand(t, "mx.dequantize")
-    device, rows, k = t.codes.device, t.codes.shape[0], t.k
+    layout = t._layout("mx.dequantize")
+    device, rows, k = t.device, t.rows, t.k
     out = torch.empty(rows, k, dtype=dtype, device=device)
-    _call(_lib.lib().dm_mx_dequantize, "mx_dequantize", device, codes, ldc, scales, lds, rows, k, FORMATS[t.fmt], out.data_ptr(), k, _DTYPES[dtype])
+    _call(_lib.lib().dm_mx_dequantize, "mx_dequantize", device, *layout, rows, k, FORMATS[t.fmt], out.data_ptr(), k, _DTYPES[dtype])
     return out
 
 
@@ -190,9 +207,8 @@ def _norm(what, kind, x, weight, bias, residual, eps, out_format):
         y = torch.empty(rows, c, dtype=dtype, device=device)
         bits, y_ptr, ldy, ys_ptr, ldys = 0, y.data_ptr(), c, None, 0
     else:
-        bits, kp = _format(out_format), _padded(c)
-        y = _new(rows, c, out_format, device)
-        y_ptr, ldy, ys_ptr, ldys = y.codes.data_ptr(), kp * bits // 8, y.scales.data_ptr(), kp // BLOCK
+        bits = _format(out_format)
+        y, y_ptr, ldy, ys_ptr, ldys = MXTensor._empty(rows, c, out_format, bits, device)
     d = RowNormDesc(x.data_ptr(), _ld(x, rows, c), r_ptr, ldr, h_ptr, c, _vector(weight, c, device, what, "weight"),
                     _vector(bias, c, device, what, "bias"), y_ptr, ldy, ys_ptr, ldys, rows, c, _DTYPES[dtype], kind, bits, eps)
     _call(_lib.lib().dm_row_norm, "row_norm", device, byref(d))
@@ -239,13 +255,13 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
         else:
             x = quantize(x, x_format)
     if x_src == _lib.X_MX:
-        bits, m, k, device = FORMATS[x.fmt], x.codes.shape[0], x.k, x.codes.device
-        x_ptr, ldx, xs_ptr, ld_xs = _operand(x, what)
+        bits, m, k, device = FORMATS[x.fmt], x.rows, x.k, x.device
+        x_ptr, ldx, xs_ptr, ld_xs = x._layout(what)
     if k != w.k:
         raise RuntimeError(f"{what}: x has rows of {k} values, w of {w.k}")
-    if device != w.codes.device:
-        raise RuntimeError(f"{what}: x is on {device}, w on {w.codes.device}")
-    n = w.codes.shape[0]
+    if device != w.device:
+        raise RuntimeError(f"{what}: x is on {device}, w on {w.device}")
+    n = w.rows
     if n < 1 or (activation == "geglu" and n % 2):
         raise RuntimeError(f"{what}: {n} output columns" + (" cannot be halved for geglu" if n else ""))
     wide = n // 2 if activation == "geglu" else n
@@ -264,10 +280,9 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
     else:
         if residual is not None:
             raise RuntimeError(f"{what}: a quantised result takes no residual")
-        c_type, kp = _format(out_format), _padded(wide)
-        y = _new(m, wide, out_format, device)
-        c_ptr, ldc, cs_ptr, ld_cs = y.codes.data_ptr(), kp * c_type // 8, y.scales.data_ptr(), kp // BLOCK
-    d = MxGemmDesc(x_ptr, ldx, xs_ptr, ld_xs, *_operand(w, what), bits, FORMATS[w.fmt], x_src, m, n, k, _vector(bias, n, device, what, "bias"),
+        c_type = _format(out_format)
+        y, c_ptr, ldc, cs_ptr, ld_cs = MXTensor._empty(m, wide, out_format, c_type, device)
+    d = MxGemmDesc(x_ptr, ldx, xs_ptr, ld_xs, *w._layout(what), bits, FORMATS[w.fmt], x_src, m, n, k, _vector(bias, n, device, what, "bias"),
                    r_ptr, ldr, c_ptr, ldc, cs_ptr, ld_cs, c_type, _ACTIVATIONS[activation])
     _call(_lib.lib().dm_mx_gemm, "mx_gemm", device, byref(d))
     return y
