@@ -152,14 +152,15 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     static constexpr int LDS = STAGES * STAGE + GROUPS * GROUP;
     static constexpr int PX = BM * XB / 1024 / WAVES, PW = BN * WB / 1024 / WAVES;  // requests of a wave's 64 lanes per k-tile
     static constexpr int LOADS = PX + PW + 1;
+    static constexpr int BLOCKS = 160 * 1024 / LDS >= 2 ? 2 : 1;  // per CU, by LDS: leave registers for as many
     static_assert(BM % 64 == 0 && BN % 64 == 0 && WM % 32 == 0 && WN % 32 == 0, "whole requests and fragments");
-    static_assert(PX * WAVES * 1024 == BM * XB && PW * WAVES * 1024 == BN * WB && BM == BN && (BM + BN) / 64 <= WAVES, "every wave requests the same");
+    static_assert(PX * WAVES * 1024 == BM * XB && PW * WAVES * 1024 == BN * WB && (BM + BN) / 64 <= WAVES, "every wave requests the same");
     static_assert(WN % 64 == 0, "a wave holds both the values and the gates of its columns");
     static_assert((STAGES - 1) * LOADS <= 63 && STAGES >= 2 && STAGES <= 4, "vmcnt counts to 63");
 };
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::WAVES)) void mx_gemm_kernel(MxArgs p) {
+__global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::WAVES), (MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::WAVES * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::BLOCKS + 3) / 4) void mx_gemm_kernel(MxArgs p) {
     typedef MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES> G;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, fr = lane & 31;
@@ -222,26 +223,27 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
         wbase += G::WB;
     };
 
-    // quarter q = 4 group + c: rows c (BM + BN) / 4 .. of the group's buffer [row][16 bytes], 16 rows per wave and four lanes per
-    // row (a second set of waves repeats the first's); c = 0, 1 are rows of X, 2, 3 rows of W.  Computed without a branch or an indexed register: the loop below is one block.
+    // quarter q = 4 group + c: rows c (BM + BN) / 4 .. of the group's buffer [row][16 bytes], 16 rows of X or of W per wave and four
+    // lanes per row (waves past the quarter's end repeat others' rows).  Computed without a branch or an indexed register: the
+    // loop below is one block.
     unsigned char* const scales = smem + STAGES * G::STAGE;
     constexpr int QUARTER = (BM + BN) / 4;
-    const int qwave = wave % (QUARTER / 16), qrow = qwave * 16 + (lane >> 2);
-    const uint32_t xs0 = (uint32_t)min(qrow, rows_left) * (uint32_t)p.ld_xs, xs1 = (uint32_t)min(QUARTER + qrow, rows_left) * (uint32_t)p.ld_xs;
-    const uint32_t ws0 = (uint32_t)w_col(qrow) * (uint32_t)p.ld_ws, ws1 = (uint32_t)w_col(QUARTER + qrow) * (uint32_t)p.ld_ws;
-    const uint32_t xs_odd = xs0 ^ xs1, ws_odd = ws0 ^ ws1;
+    const int qwave = wave % (QUARTER / 16);
     const uint64_t xscales = (uint64_t)(p.xs + (long)m0 * p.ld_xs), wscales = (uint64_t)(p.ws + (long)first * p.ld_ws);
     const uint64_t gate_scales = geglu ? (uint64_t)(p.n_out * p.ld_ws) : 0;
+    const uint32_t ld_xs = (uint32_t)p.ld_xs, ld_ws = (uint32_t)p.ld_ws;
     int quarter = 0, fill = 0;  // next quarter to request and its group's buffer
     const int last_kt = p.nkt - 1;
     auto request_scales = [&]() {
-        const uint32_t odd = quarter & 1, of_w = (quarter >> 1) & 1;
-        const uint32_t is_gate = ((odd * QUARTER + qwave * 16) >> 5) & 1;
+        const int row0 = (quarter & 3) * QUARTER + qwave * 16, row = row0 + (lane >> 2);
+        const uint32_t of_w = (uint32_t)((BM - 1 - row0) >> 31);  // all ones or zero, as the whole 16 rows are
+        const uint32_t is_gate = ((uint32_t)(row0 - BM) >> 5) & 1;
         const uint64_t wsrc = wscales + (gate_scales & (0 - (uint64_t)is_gate));
-        const uint64_t src = xscales ^ ((xscales ^ wsrc) & (0 - (uint64_t)of_w));
-        const uint32_t xoff = xs0 ^ (xs_odd & (0 - odd)), woff = ws0 ^ (ws_odd & (0 - odd));
+        const uint64_t src = xscales ^ ((xscales ^ wsrc) & ((uint64_t)of_w << 32 | of_w));
+        const uint32_t xrow = min(row, rows_left), wrow = w_col(row - BM);
         const uint32_t at = 4 * min((quarter & ~3) + (lane & 3), last_kt);  // quarters behind the last k-tile repeat it, unread
-        to_lds4((const unsigned char*)src + ((xoff ^ ((xoff ^ woff) & (0 - of_w))) + at), scales + fill * G::GROUP + ((quarter & 3) * QUARTER + qwave * 16) * 16);
+        const uint32_t off = (xrow ^ ((xrow ^ wrow) & of_w)) * (ld_xs ^ ((ld_xs ^ ld_ws) & of_w)) + at;
+        to_lds4((const unsigned char*)src + off, scales + fill * G::GROUP + row0 * 16);
         if ((++quarter & 3) == 0) fill = fill + 1 == G::GROUPS ? 0 : fill + 1;
     };
 
@@ -399,25 +401,26 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }
-// Which tile: measured over m = 1 .. 16384, n, k = 320, 1280, 5120 and 8192^2 (e4m3 x e2m1, bf16 result).
-//   256 x 256  one block per CU; 1.1 to 1.3 times the rate of the next where its rounds over the 256 CUs are full
-//              (16384 x 5120 x 5120: 343 us against 414; 4096 x 5120 x 5120, 1.25 rounds: 131 against 109)
-//   128 x 128  two blocks per CU; with waves of 32 x 64 below ten k-tiles, where the epilogue's latency counts
-//              (16384 x 5120 x 320: 63 us against 71), of 64 x 64 above (4096 x 5120 x 5120: 109 against 113)
-//   64 x 64    while the 128 x 128 tiles do not fill the chip twice, or once for a long k
-//              (1024 x 5120 x 1280: 14.0 us against 14.8; 1024 x 1280 x 5120: 22.7 against 27.8, x 5120 x 5120: 46 against 39)
+// Which tile: measured over m = 1024 .. 65536, n = 1280 .. 5120, k = 320, 1280, 5120 (e4m3 x e2m1, bf16 result) and at 8192^3.
+//   256 x 256  one block per CU.  Where its rounds over the 256 CUs are full and k is long: 8192^3 in 313 us against 381 for
+//              the next (4 bits), 437 against 459 (e4m3 x e2m1); 65536 x 2560 x 1280: 259 against 254
+//   128 x 256  two blocks per CU, so that one's epilogue runs beside the other's k loop; W in 4 bits only, whose four
+//              fragments per wave fit the 128 registers that leaves (16384 x 5120 x 320: 61 us against 68 for 256 x 256 and 79 for
+//              128 x 128; x 1280: 122, 129, 138)
+//   128 x 128  two blocks per CU, once there are enough of them, or half as many for a long k
+//   64 x 64    the rest (1024 x 5120 x 1280: 13.9 us against 14.2; 1024 x 1280 x 5120: 22.6 against 28.1)
 template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_t s) {
     const int wide = p.epi == DM_EPI_GEGLU ? 2 * p.n_pad : p.n_pad;
-    auto tiles = [&](int t) { return (long)((p.m + t - 1) / t) * ((wide + t - 1) / t); };
+    auto tiles = [&](int bm, int bn) { return (long)((p.m + bm - 1) / bm) * ((wide + bn - 1) / bn); };
     if constexpr (!EXACT) {
-        const long t256 = tiles(256), rounds = (t256 + 255) / 256;
-        if (t256 * 5 >= rounds * 256 * 4) return launch<XF, WF, EXACT, 256, 256, 128, 64, XF == 4 && WF == 4 ? 3 : 2>(p, s);
+        const long t256 = tiles(256, 256), rounds = (t256 + 255) / 256;
+        if (t256 * 5 >= rounds * 256 * 4 && (WF == 8 || p.nkt >= 32))
+            return launch<XF, WF, EXACT, 256, 256, 128, 64, XF == 4 && WF == 4 ? 3 : 2>(p, s);
+        if constexpr (WF == 4)
+            if (tiles(128, 256) >= 512) return launch<XF, WF, EXACT, 128, 256, 32, 128, 2>(p, s);
     }
-    const long t128 = tiles(128);
-    if (t128 >= 512 || (t128 >= 256 && p.nkt >= 20)) {
-        if (p.nkt < 10 || EXACT) return launch<XF, WF, EXACT, 128, 128, 32, 64, 2>(p, s);
-        return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
-    }
+    const long t128 = tiles(128, 128);
+    if (t128 >= 512 || (t128 >= 256 && p.nkt >= 20)) return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
     return launch<XF, WF, EXACT, 64, 64, 32, 64, 2>(p, s);
 }
 template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream_t s) {

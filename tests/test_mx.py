@@ -534,7 +534,7 @@ def test_feed_forward_on_another_stream_and_in_a_graph(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
-@pytest.mark.parametrize("m,n,k", [(4000, 3700, 160), (2050, 4200, 1400), (1100, 9000, 40)])
+@pytest.mark.parametrize("m,n,k", [(4000, 3700, 160), (4000, 3700, 4100), (4200, 4100, 200), (2050, 4200, 1400), (1100, 9000, 40)])
 @pytest.mark.parametrize("activation,out", [(None, torch.bfloat16), ("geglu", "mxfp8"), ("quick_gelu", torch.float32)], ids=["bf16", "geglu-mx8", "gelu-f32"])
 def test_linear_tiles_of_large_products(dev, xf, wf, m, n, k, activation, out):
     """Sizes at which the large tiles are taken, with ragged edges on all sides; 64-bit reference on the device."""
