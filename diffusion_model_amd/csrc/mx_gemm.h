@@ -28,6 +28,33 @@ struct MxArgs {
 
 __device__ __forceinline__ i32x8 widen(const i32x8& v) { return v; }
 __device__ __forceinline__ i32x8 widen(const i32x4& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }  // the instruction reads four registers
+// Also waits for this wave's LDS reads: what follows is the barrier behind which other waves refill what they read.
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+// at most min(young, MAXY) k-tiles of LOADS requests each may still be outstanding
+template <int LOADS, int MAXY> __device__ __forceinline__ void wait_young(int young) {
+    if constexpr (MAXY == 0) {
+        wait_vm<0>();
+    } else {
+        if (young >= MAXY) wait_vm<MAXY * LOADS>();
+        else wait_young<LOADS, MAXY - 1>(young);
+    }
+}
+__device__ __forceinline__ void to_lds16(const unsigned char* src, unsigned char* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(const unsigned char* src, unsigned char* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+
+// A k-tile of a row in LDS: 128 values in 128 (e4m3) or 64 (e2m1) bytes, as 16-byte chunks that the XOR below spreads over the
+// banks: any eight consecutive rows occupy eight different 16-byte columns of a 128-byte line.  Requests fill LDS lane by lane, so
+// it is the chunk they fetch that is permuted.
+template <int F> __device__ __forceinline__ int swizzle(int row, int chunk) {
+    return F == 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
+}
+template <int F> __device__ __forceinline__ i32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
+    return *reinterpret_cast<const i32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F>(row, chunk) * 16);
+}
 // A block's 32 values as bf16 with the scale applied (exact: at most four significant bits), in four groups of eight.
 template <int F> __device__ __forceinline__ void decode_block(const typename MxFragment<F>::type& c, float scale, u32x4* out) {
 #pragma unroll
@@ -66,6 +93,6 @@ __device__ __forceinline__ float gelu_poly_f(float x) {
     return x * fmaf(c, q, 0.5f);
 }
 
-// Launches the split kernel on tiles of 16 fm rows by 16 fn rows of W; fm, fn = 1 x 1, 1 x 2, 1 x 4, 2 x 2 or 2 x 4 (1 x .. where X is
+// Launches the split kernel on tiles of 16 fm rows by 16 fn rows of W; fm, fn = 1 x 1, 1 x 2, 1 x 4, 2 x 2, 2 x 4 or 4 x 4 (1 x .. where X is
 // plain rows), fn even for GEGLU, whole MX blocks of columns for an MX result.
 int dm_mx_split_launch(const MxArgs& p, int x_fmt, int w_fmt, bool exact, int x_src, int fm, int fn, hipStream_t stream);

@@ -9,36 +9,10 @@
 
 namespace {
 
-// Also waits for this wave's LDS reads: what follows is the barrier behind which other waves refill what they read.
-template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
-// at most min(young, MAXY) k-tiles of LOADS requests each may still be outstanding
-template <int LOADS, int MAXY> __device__ __forceinline__ void wait_young(int young) {
-    if constexpr (MAXY == 0) {
-        wait_vm<0>();
-    } else {
-        if (young >= MAXY) wait_vm<MAXY * LOADS>();
-        else wait_young<LOADS, MAXY - 1>(young);
-    }
-}
-__device__ __forceinline__ void to_lds16(const unsigned char* src, unsigned char* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
-__device__ __forceinline__ void to_lds4(const unsigned char* src, unsigned char* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
-}
-
 // ---- one k-tile of a 32-row operand fragment -------------------------------------------------------------------------
-// A k-tile is 128 values = blocks 0..3 of a row: 128 bytes (e4m3) or 64 (e2m1), in 16-byte chunks that the XOR below spreads
-// over the LDS banks (any eight consecutive rows then occupy eight different 16-byte columns of a 128-byte line).  Instruction
-// j = 0, 1 of a k-tile multiplies two blocks, one per lane half g = lane / 32: block 2 g + j, so that a lane's two scale bytes
-// are neighbours (one 16-bit read; the instruction selects byte j).  An e2m1 lane holds its whole block; an e4m3 lane holds
-// half g of both blocks (registers 0-3: the block of lanes 0-31).
-template <int F> __device__ __forceinline__ int swizzle(int row, int chunk) {
-    return F == 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
-}
-template <int F> __device__ __forceinline__ i32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
-    return *reinterpret_cast<const i32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F>(row, chunk) * 16);
-}
+// Instruction j = 0, 1 of a k-tile (blocks 0..3 of a row) multiplies two blocks, one per lane half g = lane / 32: block 2 g + j, so
+// that a lane's two scale bytes are neighbours (one 16-bit read; the instruction selects byte j).  An e2m1 lane holds its whole
+// block; an e4m3 lane holds half g of both blocks (registers 0-3: the block of lanes 0-31).
 // EXACT: both formats as the plain block 2 g + j, for products in bf16.
 template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type lds_fragment(const unsigned char* base, int row, int g, int j) {
     if constexpr (F == 8) {
@@ -429,14 +403,16 @@ template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream
     return launch_fmt<XF, WF, false>(p, s);
 }
 // The split kernel's tile: the smallest that needs at most one block per CU, since blocks read their operands anew
-// (64 x 1280 x 5120: 10.6 us in 320 blocks, 8.2 in 160; 16 x 8192 x 8192: 15.7 in 512, 11.7 in 256, the tile kernel 29).  Up to
-// 16 rows it is taken at any size: W is read once then, and that is all there is to do.
+// (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.1 in 200, the 64 x 64 tile 17; 512 x 1280 x 5120 with the largest 10.5 against 17.6;
+// 256 x 8192 x 8192 in 512 of those 33 against 36, 1024 x 1280 x 5120 in 320 of them 23 against 22).  The largest is slower than
+// the 64 x 64 tile on a short k (512 x 1280 x 320: 5.2 us against 4.5).  Up to 16 rows a tile of 16 x 64 is taken at any size: W
+// is read once then, and that is all there is to do.
 bool split_tile(const MxArgs& p, int* fm, int* fn) {
-    static const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {1, 4}};
+    static const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {1, 4}, {2, 4}, {4, 4}};
     const bool geglu = p.epi == DM_EPI_GEGLU, mx = p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4;
     for (const auto& t : shapes) {
         const int cols = geglu ? t[1] * 8 : t[1] * 16;
-        if ((geglu && t[1] % 2) || (mx && cols % MX_BLOCK) || (t[0] > 1 && p.m <= 16)) continue;
+        if ((geglu && t[1] % 2) || (mx && cols % MX_BLOCK) || (t[0] > 1 && p.m <= 16) || (t[0] == 4 && p.nkt < 8)) continue;
         const long blocks = (long)((p.m + 16 * t[0] - 1) / (16 * t[0])) * ((p.n_pad + cols - 1) / cols);
         if (blocks <= 256 || (p.m <= 16 && t[1] == 4)) {
             *fm = t[0];

@@ -3,15 +3,15 @@
 
 namespace {
 
-// ---- split kernel ----------------------------------------------------------------------------------------------------
 // Few output tiles: the eight waves of a block share one tile of 16 FM rows by 16 FN rows of W; every eighth k-tile is a wave's, so
-// that their reads of a row lie side by side.  Nothing is
-// shared before the end, so operands go from memory straight to registers, UNIT k-tiles at once and without a barrier, and the
-// eight partial sums meet in LDS in a fixed order.  What bounds it is how many cache lines the loads touch, so it uses the
-// 16-row instruction: four lanes read 64 bytes of a row where the 32-row one's two lanes read 32, and the scales of four
-// k-tiles come as 16 bytes of a row by its four lanes, which hand them round (16 x 8192 x 8192: x us against y).
-// XSRC: 0 = X is an MX matrix, 1 / 2 = X is bf16 / fp32 rows that every block quantises as it reads them, to the codes that
-// dm_mx_quantize gives: a block's 32 values are in one lane or in a pair of them.
+// that their reads of a row lie side by side, and the eight partial sums meet in LDS in a fixed order.  Until then nothing is
+// shared: each wave keeps a ring of DEPTH k-tiles in LDS of its own and waits for nobody.
+// Fragments are not loaded straight to registers: the instruction wants 16 rows in 16 neighbouring lanes, and such a load
+// costs a pass per row and quarter wave (measured 61 cycles for 1 KB; 16 x 8192 x 8192 took 11.2 us so, at 14 bytes per cycle and CU
+// whatever cache held them).  A request with four or eight lanes to a row does not: 7.6 us through LDS, 36 MB at 4.8 TB/s with the
+// launch's 2.5 us in it; 77 x 1280 x 5120 5.0 us against 8.2 (and 17 for the 64 x 64 tile).
+// x_src: X is an MX matrix, or bf16 / fp32 rows that every block quantises as it reads them, a block of 32 values per lane, to
+// the codes that dm_mx_quantize gives.
 constexpr int SPLIT_WAVES = 8;
 
 // N values from p on, those at `left` and behind as zeros
@@ -25,48 +25,35 @@ template <typename T, int N> __device__ __forceinline__ void load_values(const T
         for (int i = 0; i < N; ++i) v[i] = i < left ? ElemTraits<T>::load(p + i) : 0.f;
     }
 }
-// A lane's share of a 16-row operand of one instruction (128 values per row, four lanes g to a row).  e2m1, or EXACT: block g;
-// e4m3: 16 values from 16 g (registers 0-3) and from 64 + 16 g on.  Its scale operand is that of block g either way.
-template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type load_fragment16(const unsigned char* at, int g) {
+// A lane's share of a 16-row operand of one instruction (128 values per row, four lanes g to a row), from the row in LDS.  e2m1, or
+// EXACT: block g; e4m3: 16 values from 16 g (registers 0-3) and from 64 + 16 g on.  Its scale operand is that of block g either way.
+template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type lds_fragment16(const unsigned char* base, int row, int g) {
     if constexpr (F == 8) {
-        const i32x4 lo = *reinterpret_cast<const i32x4*>(at + (EXACT ? 32 * g : 16 * g));
-        const i32x4 hi = *reinterpret_cast<const i32x4*>(at + (EXACT ? 32 * g + 16 : 64 + 16 * g));
+        const i32x4 lo = lds_chunk<8>(base, row, EXACT ? 2 * g : g);
+        const i32x4 hi = lds_chunk<8>(base, row, EXACT ? 2 * g + 1 : 4 + g);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-        return *reinterpret_cast<const i32x4*>(at + 16 * g);
+        return lds_chunk<4>(base, row, g);
     }
 }
-template <int F, bool EXACT, typename T>
-__device__ __forceinline__ typename MxFragment<F>::type quantize_fragment16(const T* row, int k, int kt, int lane, int& scale) {
-    const int g = lane >> 4;
-    typename MxFragment<F>::type out;
+// One k-tile of 16 plain rows -> codes [16][k-tile] and scales (byte `word` * 4 + block of [16][16]) in LDS: lane (row, block)
+template <int F, typename T>
+__device__ __forceinline__ void quantize_tile16(const T* row, int k, int kt, int lane, unsigned char* codes, unsigned char* scales, int word) {
+    const int r = lane >> 2, block = lane & 3, at = kt * MX_PAD + 32 * block;
     float v[32];
-    uint32_t byte[2];
-    if constexpr (F == 8 && !EXACT) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {  // half a block each; the other half is in lane l ^ 16
-            const int at = kt * MX_PAD + 64 * b + 16 * g;
-            load_values<T, 16>(row + at, k - at, v + 16 * b);
-            float top = mx_largest<16>(v + 16 * b);
-            top = __builtin_elementwise_maximum(top, __shfl_xor(top, 16));
-            byte[b] = mx_scale_byte<8>(top);  // of block 2 b + g / 2
-        }
-        const int from = (lane & 15) + 32 * (g & 1);  // a lane that holds the byte of block g
-        const int lo = __shfl((int)byte[0], from), hi = __shfl((int)byte[1], from);
-        scale = g < 2 ? lo : hi;
-    } else {
-        const int at = kt * MX_PAD + 32 * g;
-        load_values<T, 32>(row + at, k - at, v);
-        byte[0] = byte[1] = mx_scale_byte<F>(mx_largest<32>(v));
-        scale = (int)byte[0];
-    }
+    load_values<T, 32>(row + at, k - at, v);
+    const uint32_t byte = mx_scale_byte<F>(mx_largest<32>(v));
+    uint32_t w[4 * MxCodes<F>::W];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const MxCodes<F> c = mx_encode8<F>(v + 8 * q, byte[q >> 1]);
+        const MxCodes<F> c = mx_encode8<F>(v + 8 * q, byte);
 #pragma unroll
-        for (int e = 0; e < MxCodes<F>::W; ++e) out[q * MxCodes<F>::W + e] = (int)c.w[e];
+        for (int e = 0; e < MxCodes<F>::W; ++e) w[q * MxCodes<F>::W + e] = c.w[e];
     }
-    return out;
+#pragma unroll
+    for (int c = 0; c < MxCodes<F>::W; ++c)
+        *reinterpret_cast<u32x4*>(codes + r * mx_bytes(F, MX_PAD) + swizzle<F>(r, block * MxCodes<F>::W + c) * 16) = u32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
+    scales[r * 16 + word * 4 + block] = (unsigned char)byte;
 }
 template <int XF, int WF, bool EXACT>
 __device__ __forceinline__ void mma16(f32x4& acc, const typename MxFragment<XF>::type& x, const typename MxFragment<WF>::type& w, int sx, int sw) {
@@ -122,82 +109,129 @@ __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* 
     }
 }
 
+template <int XF, int WF, int FM, int FN> struct SplitRing {
+    static constexpr int XB = mx_bytes(XF, MX_PAD), WB = mx_bytes(WF, MX_PAD);
+    static constexpr int TILE = 16 * (FM * XB + FN * WB);  // bytes of a k-tile
+    static constexpr int DEPTH = SPLIT_WAVES * TILE * 4 <= 128 * 1024 ? 4 : SPLIT_WAVES * TILE * 2 <= 128 * 1024 ? 2 : 1;
+    static constexpr int GROUP = 16 * (FM + FN) * 16;  // scales of four k-tiles: [row][16 bytes]; two such buffers
+    static constexpr int WAVE = DEPTH * TILE + 2 * GROUP;
+    static constexpr int LDS = SPLIT_WAVES * (WAVE > FM * FN * 1024 ? WAVE : FM * FN * 1024);  // the partial sums reuse it
+    static constexpr int XN = XB / 64, WN = WB / 64;  // requests per fragment: 8 or 16 rows each
+    static_assert(LDS <= 160 * 1024, "LDS of a CU");
+};
+
 template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN>
 __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
+    typedef SplitRing<XF, WF, FM, FN> G;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 4, fr = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool geglu = p.epi == DM_EPI_GEGLU;
-    constexpr int UNIT = FM * FN <= 2 ? 4 : 2;  // k-tiles whose operands are on their way together
     const int tile_m = blockIdx.x / p.tiles_n, tile_n = blockIdx.x % p.tiles_n;
     const int m0 = tile_m * 16 * FM, col0 = tile_n * (geglu ? FN * 8 : FN * 16);
 
-    // rows that do not exist are read from the last one
-    const unsigned char *xrow[FM], *xsrow[FM], *wrow[FN], *wsrow[FN];
+    // ---- sources: 16-byte pieces of rows by eight (e4m3) or four lanes, scale words by four.  Rows that do not exist are read
+    // from the last one.
+    auto x_row = [&](int r) { return (long)min(m0 + r, p.m - 1); };
+    auto w_row = [&](int j, int r) {  // GEGLU: fragments 0, 2, .. are values, 1, 3, .. their gates
+        return (long)min(col0 + (geglu ? j >> 1 : j) * 16 + r, p.n_out - 1) + (geglu && (j & 1) ? p.n_out : 0);
+    };
+    const unsigned char *xp[FM][G::XN], *wp[FN][G::WN], *xsp[FM], *wsp[FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const long row = min(m0 + i * 16 + fr, p.m - 1);
-        xrow[i] = p.x + row * p.ldx;
-        xsrow[i] = XSRC == 0 ? p.xs + row * p.ld_xs : nullptr;
+        if constexpr (XSRC == DM_X_MX) {
+#pragma unroll
+            for (int e = 0; e < G::XN; ++e) {
+                const int r = e * (16 / G::XN) + lane / (G::XB / 16), pos = lane % (G::XB / 16);
+                xp[i][e] = p.x + x_row(i * 16 + r) * p.ldx + swizzle<XF>(r, pos) * 16;
+            }
+            xsp[i] = p.xs + x_row(i * 16 + (lane >> 2)) * p.ld_xs;
+        } else {
+            xp[i][0] = p.x + x_row(i * 16 + (lane >> 2)) * p.ldx;
+        }
     }
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {  // GEGLU: fragments 0, 2, .. are values, 1, 3, .. their gates
-        const long row = min(col0 + (geglu ? j >> 1 : j) * 16 + fr, p.n_out - 1) + (geglu && (j & 1) ? p.n_out : 0);
-        wrow[j] = p.w + row * p.ldw;
-        wsrow[j] = p.ws + row * p.ld_ws;
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+        for (int e = 0; e < G::WN; ++e) {
+            const int r = e * (16 / G::WN) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
+            wp[j][e] = p.w + w_row(j, r) * p.ldw + swizzle<WF>(r, pos) * 16;
+        }
+        wsp[j] = p.ws + w_row(j, lane >> 2) * p.ld_ws;
     }
+    const int count = (p.nkt - wave + SPLIT_WAVES - 1) / SPLIT_WAVES;  // this wave's k-tiles: wave, wave + 8, ..
+    unsigned char* const ring = smem + wave * G::WAVE;
+    unsigned char* const groups = ring + G::DEPTH * G::TILE;
+    auto request = [&](int s, int slot) {
+        const int kt = wave + SPLIT_WAVES * s;
+        unsigned char* const group = groups + ((s >> 2) & 1) * G::GROUP;
+        if ((s & 3) == 0) {  // scale words of this k-tile and the wave's next three (the last one repeated)
+            const int at = 4 * (wave + SPLIT_WAVES * min(s + (lane & 3), count - 1));
+#pragma unroll
+            for (int j = 0; j < FN; ++j) to_lds4(wsp[j] + at, group + (FM + j) * 256);
+            if constexpr (XSRC == DM_X_MX) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i) to_lds4(xsp[i] + at, group + i * 256);
+            }
+        }
+        unsigned char* const to = ring + slot * G::TILE;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < G::WN; ++e) to_lds16(wp[j][e] + (long)kt * G::WB, to + FM * 16 * G::XB + (j * G::WN + e) * 1024);
+        if constexpr (XSRC == DM_X_MX) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int e = 0; e < G::XN; ++e) to_lds16(xp[i][e] + (long)kt * G::XB, to + (i * G::XN + e) * 1024);
+        }
+    };
+    constexpr int LOADS = FN * G::WN + (XSRC == DM_X_MX ? FM * G::XN : 0);  // per k-tile; scale words on top only lengthen a wait
+
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{};
-
-    auto process = [&](int kt, auto count) {
-        constexpr int N = decltype(count)::value;  // k-tiles kt, kt + 8, .. of this wave
-        typename MxFragment<XF>::type x[N][FM];
-        typename MxFragment<WF>::type w[N][FN];
-        int sx[N][FM], sw[N][FN], sxw[FM], sww[FN];
-        // lane g: the four scale bytes of k-tile g (mod N) of its row
-        const long sat = 4L * (kt + SPLIT_WAVES * (g % N));
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sww[j] = *reinterpret_cast<const int*>(wsrow[j] + sat);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-            if constexpr (XSRC == 0) sxw[i] = *reinterpret_cast<const int*>(xsrow[i] + sat);
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-#pragma unroll
-            for (int j = 0; j < FN; ++j) w[u][j] = load_fragment16<WF, EXACT>(wrow[j] + (long)(kt + SPLIT_WAVES * u) * mx_bytes(WF, MX_PAD), g);
+    for (int s = 0; s < G::DEPTH; ++s)
+        if (s < count) request(s, s);
+    int slot = 0;
+    for (int s = 0; s < count; ++s) {
+        unsigned char* const at = ring + slot * G::TILE;
+        unsigned char* const group = groups + ((s >> 2) & 1) * G::GROUP;
+        if constexpr (XSRC != DM_X_MX) {
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                if constexpr (XSRC == 0) x[u][i] = load_fragment16<XF, EXACT>(xrow[i] + (long)(kt + SPLIT_WAVES * u) * mx_bytes(XF, MX_PAD), g);
-                if constexpr (XSRC == 1) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const bf16_t*>(xrow[i]), p.k, kt + SPLIT_WAVES * u, lane, sx[u][i]);
-                if constexpr (XSRC == 2) x[u][i] = quantize_fragment16<XF, EXACT>(reinterpret_cast<const float*>(xrow[i]), p.k, kt + SPLIT_WAVES * u, lane, sx[u][i]);
+                typedef typename std::conditional<XSRC == DM_X_F32, float, bf16_t>::type T;
+                quantize_tile16<XF, T>(reinterpret_cast<const T*>(xp[i][0]), p.k, wave + SPLIT_WAVES * s, lane, at + i * 16 * G::XB, group + i * 256, s & 3);
             }
         }
+        wait_young<LOADS, G::DEPTH - 1>(count - 1 - s);  // k-tile s has landed; nobody else reads or writes this ring
+        typename MxFragment<XF>::type x[FM];
+        typename MxFragment<WF>::type w[FN];
+        int sx[FM], sw[FN];
 #pragma unroll
-        for (int u = 0; u < N; ++u) {  // byte g of the word that lane u of the row holds
-#pragma unroll
-            for (int j = 0; j < FN; ++j) sw[u][j] = (N == 1 ? sww[j] : __shfl(sww[j], u * 16 + fr)) >> (8 * g);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                if constexpr (XSRC == 0) sx[u][i] = (N == 1 ? sxw[i] : __shfl(sxw[i], u * 16 + fr)) >> (8 * g);
+        for (int i = 0; i < FM; ++i) {
+            x[i] = lds_fragment16<XF, EXACT>(at + i * 16 * G::XB, fr, g);
+            sx[i] = group[i * 256 + fr * 16 + (s & 3) * 4 + g];
         }
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) mma16<XF, WF, EXACT>(acc[i][j], x[u][i], w[u][j], sx[u][i], sw[u][j]);
-    };
-    int kt = wave;
-    for (; kt + SPLIT_WAVES * (UNIT - 1) < p.nkt; kt += SPLIT_WAVES * UNIT) process(kt, std::integral_constant<int, UNIT>());
-    if constexpr (UNIT == 4)
-        if (kt + SPLIT_WAVES < p.nkt) {
-            process(kt, std::integral_constant<int, 2>());
-            kt += 2 * SPLIT_WAVES;
+        for (int j = 0; j < FN; ++j) {
+            w[j] = lds_fragment16<WF, EXACT>(at + FM * 16 * G::XB + j * 16 * G::WB, fr, g);
+            sw[j] = group[(FM + j) * 256 + fr * 16 + (s & 3) * 4 + g];
         }
-    if (kt < p.nkt) process(kt, std::integral_constant<int, 1>());
+        if (s + G::DEPTH < count) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments are in registers: the slot may be refilled
+            request(s + G::DEPTH, slot);
+        }
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) mma16<XF, WF, EXACT>(acc[i][j], x[i], w[j], sx[i], sw[j]);
+        if (++slot == G::DEPTH) slot = 0;
+    }
+    __syncthreads();  // the rings are done with
 
     // ---- partial sums [wave][fragment][lane]; lane (q, m) of a fragment holds columns 4 q .. 4 q + 3 of row m.  A thread then
     // sums eight columns of one row: four threads to 32 columns.
@@ -238,8 +272,11 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 }
 
 template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN> int launch_split(MxArgs p, hipStream_t s) {
-    constexpr int LDS = SPLIT_WAVES * FM * FN * 1024;
-    static_assert(32 * FM * FN <= 64 * SPLIT_WAVES && LDS <= 64 * 1024, "one thread per eight columns");
+    constexpr int LDS = SplitRing<XF, WF, FM, FN>::LDS;
+    static_assert(32 * FM * FN <= 64 * SPLIT_WAVES, "one thread per eight columns");
+    static DmLdsAttr attr;
+    if (LDS > 64 * 1024)
+        if (const int rc = dm_set_lds_attr(reinterpret_cast<const void*>(&mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN>), attr, LDS)) return rc;
     const int bo = p.epi == DM_EPI_GEGLU ? FN * 8 : FN * 16;
     p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
     p.tiles_n = (p.n_pad + bo - 1) / bo;
@@ -257,6 +294,7 @@ template <int XF, int WF, bool EXACT, int XSRC> int launch_tile(const MxArgs& p,
     if constexpr (XSRC == DM_X_MX) {
         if (fm == 2 && fn == 2) return launch_split<XF, WF, EXACT, XSRC, 2, 2>(p, s);
         if (fm == 2 && fn == 4) return launch_split<XF, WF, EXACT, XSRC, 2, 4>(p, s);
+        if (fm == 4 && fn == 4) return launch_split<XF, WF, EXACT, XSRC, 4, 4>(p, s);
     }
     return DM_ERR_ARG;
 }
