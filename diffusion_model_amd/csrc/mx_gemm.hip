@@ -434,7 +434,7 @@ int operand(const void* codes, long ld, const void* scales, long lds, int kp, in
 }  // namespace
 
 extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
-    if (!d || d->m < 0 || d->n < 1 || d->k < 1 || d->k > (1 << 24) || d->n > (1 << 24) || !fmt_ok(d->x_fmt) || !fmt_ok(d->w_fmt)) return DM_ERR_ARG;
+    if (!d || d->m < 0 || d->m > (1 << 30) || d->n < 1 || d->k < 1 || d->k > (1 << 24) || d->n > (1 << 24) || !fmt_ok(d->x_fmt) || !fmt_ok(d->w_fmt)) return DM_ERR_ARG;
     if (d->epi != DM_EPI_PLAIN && d->epi != DM_EPI_GEGLU && d->epi != DM_EPI_QUICKGELU) return DM_ERR_ARG;
     if (d->epi == DM_EPI_GEGLU && d->n % 2) return DM_ERR_ARG;
     if (d->c_type != DM_F32 && d->c_type != DM_BF16 && !fmt_ok(d->c_type)) return DM_ERR_ARG;

@@ -28,6 +28,7 @@ FORMATS = {"mxfp8": _lib.DM_MXFP8, "mxfp4": _lib.DM_MXFP4}
 _DTYPES = {torch.float32: _lib.DM_F32, torch.bfloat16: _lib.DM_BF16}
 _ACTIVATIONS = {None: _lib.EPI_PLAIN, "quick_gelu": _lib.EPI_QUICKGELU, "geglu": _lib.EPI_GEGLU}
 BLOCK, PAD, MAX_K = 32, 128, 1 << 24
+MAX_ROWS, MAX_COLUMNS = 1 << 30, 1 << 24  # of a product
 
 
 def _padded(k: int) -> int:
@@ -264,6 +265,8 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
     n = w.rows
     if n < 1 or (activation == "geglu" and n % 2):
         raise RuntimeError(f"{what}: {n} output columns" + (" cannot be halved for geglu" if n else ""))
+    if m > MAX_ROWS or n > MAX_COLUMNS:
+        raise RuntimeError(f"{what}: a product of {m} x {n} is too large (at most {MAX_ROWS} x {MAX_COLUMNS})")
     wide = n // 2 if activation == "geglu" else n
     r_ptr, ldr, cs_ptr, ld_cs = None, 0, None, 0
     if out_format is None:

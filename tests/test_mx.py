@@ -136,7 +136,8 @@ def test_c_entry_points_refuse_bad_arguments_without_a_device():
             setattr(d, k, v)
         return lib.dm_mx_gemm(C.byref(d), None)
     assert lib.dm_mx_gemm(None, None) == 1 and gemm(m=0) == 0
-    for kw in (dict(x=None), dict(w_scales=None), dict(c=None), dict(ldx=112), dict(ld_ws=3), dict(x_fmt=1), dict(n=0), dict(k=0), dict(m=-1), dict(ldc=5),
+    for kw in (dict(x=None), dict(w_scales=None), dict(c=None), dict(ldx=112), dict(ld_ws=3), dict(x_fmt=1), dict(n=0), dict(k=0), dict(m=-1), dict(m=(1 << 30) + 1), dict(n=(1 << 24) + 1), dict(ldc=5), dict(ldx=(1 << 24) + 16),
+               dict(x_src=3), dict(x_src=_lib.X_BF16, ldx=99), dict(x_src=_lib.X_F32, m=17),
                dict(r=p, ldr=5), dict(epi=_lib.EPI_NCHW_F32), dict(epi=_lib.EPI_GEGLU, n=7), dict(c_type=3), dict(c_type=8, c_scales=None),
                dict(c_type=8, c_scales=p, ld_cs=4, ldc=128, r=p, ldr=8), dict(c_type=4, c_scales=p, ld_cs=4, ldc=48)):
         assert gemm(**kw) == 1, kw
@@ -442,6 +443,30 @@ def test_linear_nan_stays_in_its_row(dev, m, out):
         wb[5, 3] = math.inf
         y = mx.linear(x[3:].to(dev) if m > 3 else x[:1].to(dev), mx.quantize(wb.to(dev), "mxfp8"), x_format=xf).cpu()
         assert torch.isnan(y[:, 5]).all() and torch.isfinite(y[:, :5]).all() and torch.isfinite(y[:, 6:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
+@pytest.mark.parametrize("m,n", [(1100, 1100), (4200, 4100)])  # the tile kernels
+def test_linear_nan_stays_in_its_row_and_column_of_a_tile(dev, xf, wf, m, n):
+    x, w = torch.ones(m, 200, device=dev), torch.ones(n, 200, device=dev)
+    x[7, 150], w[33, 0] = math.nan, math.inf
+    for out in DTYPES:
+        y = mx.linear(mx.quantize(x, xf), mx.quantize(w, wf), out_dtype=out)
+        bad = torch.isnan(y)
+        assert bad[7].all() and bad[:, 33].all() and int(bad.sum()) == m + n - 1 and (y[~bad] == 200).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
+@pytest.mark.parametrize("m", [4, 1100])
+def test_linear_extreme_scales(dev, xf, wf, m):
+    """Blocks at both ends of the scales' range: 128 products 2^x 2^w, exact in every type."""
+    for ex, ew in ((-120, 120), (-60, -60), (100, -120), (-125, 126), (126, -125), (-127 + EMAX[xf], 100)):
+        x, w = torch.full((m, 128), 2.0 ** ex, device=dev), torch.full((1100, 128), 2.0 ** ew, device=dev)
+        for out in DTYPES:
+            y = mx.linear(mx.quantize(x, xf), mx.quantize(w, wf), out_dtype=out)
+            assert (y.double() == 2.0 ** (ex + ew + 7)).all(), (ex, ew, out)
 
 
 @pytest.mark.gpu
