@@ -46,68 +46,80 @@ __device__ __forceinline__ void mma_row(f32x16 (&acc)[FN], const typename MxFrag
 }
 
 // ---- epilogue --------------------------------------------------------------------------------------------------------
-// 16 consecutive columns of row m from column `col` on, in the result's type; `edge`: some of the block's are past n_out.
-template <int F> __device__ __forceinline__ void store16_mx(const MxArgs& p, long m, int col, const float* v, int lane) {
-    // lanes l and l + 32 hold the two halves of a block
-    float top = mx_largest<16>(v);
-    top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32));
-    if (m >= p.m || col >= p.n_pad) return;
-    const uint32_t byte = mx_scale_byte<F>(top);
-    const MxCodes<F> a = mx_encode8<F>(v, byte), b = mx_encode8<F>(v + 8, byte);
-    unsigned char* dst = static_cast<unsigned char*>(p.c) + m * p.ldc + mx_bytes(F, col);
-    if constexpr (F == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{a.w[0], a.w[1], b.w[0], b.w[1]};
-    else *reinterpret_cast<u32x2*>(dst) = u32x2{a.w[0], b.w[0]};
-    if (lane < 32) p.cs[m * p.ld_cs + (col >> 5)] = (unsigned char)byte;
-}
-__device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float* v, int lane, bool edge) {
-    if (p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4) {
+// 16 consecutive columns of row m from column `col` on, in the result's type CT; `edge`: some of the block's are past n_out.
+template <int CT> __device__ __forceinline__ void store16(const MxArgs& p, long m, int col, float* v, int lane, bool edge) {
+    if constexpr (CT == DM_MXFP8 || CT == DM_MXFP4) {
         if (edge) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = col + e < p.n_out ? v[e] : 0.f;
         }
-        if (p.c_type == DM_MXFP8) store16_mx<8>(p, m, col, v, lane);
-        else store16_mx<4>(p, m, col, v, lane);
-        return;
-    }
-    if (m >= p.m || col >= p.n_out) return;
-    const int left = p.n_out - col;
-    const bool whole = left >= 16;
-    if (p.c_type == DM_BF16) {
-        bf16_t* dst = static_cast<bf16_t*>(p.c) + m * p.ldc + col;
-        const bf16_t* res = static_cast<const bf16_t*>(p.r) + m * p.ldr + col;
-        if (whole) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (p.r) {
-                    float f[8];
-                    chunk_to_f32<bf16_t>(load16_any(res + 8 * h), f);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[8 * h + i] += f[i];
-                }
-                store16_any(dst + 8 * h, f32_to_chunk<bf16_t>(v + 8 * h));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < left) dst[i] = f32_to_bf16(p.r ? v[i] + bf16_to_f32(res[i]) : v[i]);
-        }
+        // lanes l and l + 32 hold the two halves of a block
+        float top = mx_largest<16>(v);
+        top = __builtin_elementwise_maximum(top, __shfl_xor(top, 32));
+        if (m >= p.m || col >= p.n_pad) return;
+        const uint32_t byte = mx_scale_byte<CT>(top);
+        const MxCodes<CT> a = mx_encode8<CT>(v, byte), b = mx_encode8<CT>(v + 8, byte);
+        unsigned char* dst = static_cast<unsigned char*>(p.c) + m * p.ldc + mx_bytes(CT, col);
+        if constexpr (CT == DM_MXFP8) *reinterpret_cast<u32x4*>(dst) = u32x4{a.w[0], a.w[1], b.w[0], b.w[1]};
+        else *reinterpret_cast<u32x2*>(dst) = u32x2{a.w[0], b.w[0]};
+        if (lane < 32) p.cs[m * p.ld_cs + (col >> 5)] = (unsigned char)byte;
     } else {
-        float* dst = static_cast<float*>(p.c) + m * p.ldc + col;
-        const float* res = static_cast<const float*>(p.r) + m * p.ldr + col;
-        if (whole) {
+        typedef typename std::conditional<CT == DM_F32, float, bf16_t>::type T;
+        constexpr int EPC = ElemTraits<T>::EPC;
+        if (m >= p.m || col >= p.n_out) return;
+        T* dst = static_cast<T*>(p.c) + m * p.ldc + col;
+        const T* res = static_cast<const T*>(p.r) + m * p.ldr + col;
+        const int left = p.n_out - col;
+        if (!edge || left >= 16) {
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                f32x4 o = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-                if (p.r) o += __builtin_bit_cast(f32x4, load16_any(res + 4 * h));
-                store16_any(dst + 4 * h, __builtin_bit_cast(u32x4, o));
+            for (int h = 0; h < 16 / EPC; ++h) {
+                if (p.r) {
+                    float f[EPC];
+                    chunk_to_f32<T>(load16_any(res + EPC * h), f);
+#pragma unroll
+                    for (int i = 0; i < EPC; ++i) v[EPC * h + i] += f[i];
+                }
+                store16_any(dst + EPC * h, f32_to_chunk<T>(v + EPC * h));
             }
         } else {
-#pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (i < left) dst[i] = p.r ? v[i] + res[i] : v[i];
+                if (i < left) ElemTraits<T>::store(dst + i, p.r ? v[i] + ElemTraits<T>::load(res + i) : v[i]);
         }
     }
 }
+// A wave's fragments.  One instance per activation and type: with the choices inside, every fragment's code holds all of them
+// and the instruction cache (64 KB for two CUs) sees the epilogue anew with each tile.
+template <int EPI, int CT, int FM, int FN, typename Row, typename Column>
+__device__ __forceinline__ void store_fragments(const MxArgs& p, const f32x16 (&acc)[FM][FN], Row row, Column column, int lane, bool edge) {
+    constexpr int STEP = EPI == DM_EPI_GEGLU ? 2 : 1;
+#pragma unroll
+    for (int j = 0; j < FN; j += STEP)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float o = acc[i][j][e];
+                if constexpr (EPI == DM_EPI_GEGLU) {
+                    const float gate = acc[i][j + STEP - 1][e];
+                    v[e] = o * (CT == DM_F32 ? gelu_erf_f(gate) : gelu_poly_f(gate));
+                } else if constexpr (EPI == DM_EPI_QUICKGELU) {
+                    v[e] = o / (1.f + __expf(-1.702f * o));
+                } else {
+                    v[e] = o;
+                }
+            }
+            store16<CT>(p, row(i), column(j), v, lane, edge);
+        }
+}
+template <int EPI, int FM, int FN, typename Row, typename Column>
+__device__ __forceinline__ void store_typed(const MxArgs& p, const f32x16 (&acc)[FM][FN], Row row, Column column, int lane, bool edge) {
+    if (p.c_type == DM_BF16) store_fragments<EPI, DM_BF16>(p, acc, row, column, lane, edge);
+    else if (p.c_type == DM_F32) store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
+    else if (p.c_type == DM_MXFP8) store_fragments<EPI, DM_MXFP8>(p, acc, row, column, lane, edge);
+    else store_fragments<EPI, DM_MXFP4>(p, acc, row, column, lane, edge);
+}
+
 // ---- tile kernel -----------------------------------------------------------------------------------------------------
 // BM rows of X by BN rows of W per block, one WM x WN piece per wave; a ring of STAGES k-tiles in LDS, filled by loads that
 // bypass the registers.  EXACT: the operands are decoded to bf16 and multiplied there (see dm_mx_gemm).
@@ -330,35 +342,10 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
 
     // ---- epilogue: a lane holds row .. + fr and 16 columns per fragment
     const bool edge = col0 + (geglu ? BN / 2 : BN) > p.n_out;
-    if (geglu) {
-#pragma unroll
-        for (int j = 0; j < FN; j += 2)
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                float v[16];
-                if (p.c_type == DM_F32) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_erf_f(acc[i][j + 1][e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * gelu_poly_f(acc[i][j + 1][e]);
-                }
-                store16(p, m0 + wm * WM + i * 32 + fr, column(j), v, lane, edge);
-            }
-    } else {
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                float v[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float o = acc[i][j][e];
-                    v[e] = p.epi == DM_EPI_QUICKGELU ? o / (1.f + __expf(-1.702f * o)) : o;
-                }
-                store16(p, m0 + wm * WM + i * 32 + fr, column(j), v, lane, edge);
-            }
-    }
+    auto row = [&](int i) { return (long)(m0 + wm * WM + i * 32 + fr); };
+    if (geglu) store_typed<DM_EPI_GEGLU>(p, acc, row, column, lane, edge);
+    else if (p.epi == DM_EPI_QUICKGELU) store_typed<DM_EPI_QUICKGELU>(p, acc, row, column, lane, edge);
+    else store_typed<DM_EPI_PLAIN>(p, acc, row, column, lane, edge);
 }
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {
