@@ -125,7 +125,7 @@ struct NormArgs {
     void* y;            // T rows, or codes
     unsigned char* ys;  // scales
     long ldx, ldr, ldh, ldy, ldys;
-    long rows;
+    long rows, first;  // rows of the matrix; row of the launch's first block
     int c, layer;
     float eps;
 };
@@ -193,7 +193,7 @@ template <typename T, int OUT, int TPR, int NV>
 __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
     __shared__ float red[TPR / 64];
     const int t = threadIdx.x % TPR;
-    const long row = (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+    const long row = p.first + (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
     if (row >= p.rows) return;  // whole waves; TPR > 64 has one row per block
     const int cp = OUT ? mx_padded(p.c) : p.c;
     float v[NV][8];
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
 // or the residual itself here as in the kernel above.
 template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_norm_loop_kernel(NormArgs p) {
     __shared__ float red[THREADS / 64];
-    const long row = blockIdx.x;
+    const long row = p.first + blockIdx.x;
     const int cp = OUT ? mx_padded(p.c) : p.c;
     const T* stored = p.r ? static_cast<const T*>(p.h) + row * p.ldh : static_cast<const T*>(p.x) + row * p.ldx;
     float s = 0.f, mean = 0.f;
@@ -278,9 +278,18 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
     }
 }
 
-template <typename T, int OUT, int TPR, int NV> int launch_row_norm(const NormArgs& p, hipStream_t s) {
-    row_norm_kernel<T, OUT, TPR, NV><<<dim3((unsigned)((p.rows + THREADS / TPR - 1) / (THREADS / TPR))), THREADS, 0, s>>>(p);
-    return dm_check_launch();
+// A launch holds fewer than 2^32 threads: longer matrices take several.
+constexpr long MAX_BLOCKS = 1L << 23;
+template <typename T, int OUT, int TPR, int NV> int launch_row_norm(NormArgs p, hipStream_t s) {
+    constexpr int ROWS = THREADS / TPR;  // per block
+    for (p.first = 0; p.first < p.rows; p.first += MAX_BLOCKS * ROWS) {
+        const long blocks = (p.rows - p.first + ROWS - 1) / ROWS;
+        const dim3 grid((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS));
+        if constexpr (NV > 0) row_norm_kernel<T, OUT, TPR, NV><<<grid, THREADS, 0, s>>>(p);
+        else row_norm_loop_kernel<T, OUT><<<grid, THREADS, 0, s>>>(p);
+        if (const int rc = dm_check_launch()) return rc;
+    }
+    return DM_OK;
 }
 template <typename T, int OUT> int launch_norm(const NormArgs& p, hipStream_t s) {
     if (p.c <= 512) return launch_row_norm<T, OUT, 64, 1>(p, s);
@@ -289,8 +298,7 @@ template <typename T, int OUT> int launch_norm(const NormArgs& p, hipStream_t s)
     if (p.c <= 4096) return launch_row_norm<T, OUT, 256, 2>(p, s);
     if (p.c <= 8192) return launch_row_norm<T, OUT, 256, 4>(p, s);
     if (p.c <= 16384) return launch_row_norm<T, OUT, 256, 8>(p, s);
-    row_norm_loop_kernel<T, OUT><<<dim3((unsigned)p.rows), THREADS, 0, s>>>(p);
-    return dm_check_launch();
+    return launch_row_norm<T, OUT, 256, 0>(p, s);
 }
 
 bool mx_fmt_ok(int fmt) { return fmt == DM_MXFP8 || fmt == DM_MXFP4; }
@@ -304,7 +312,8 @@ int mx_layout(const void* codes, long ldc, const void* scales, long lds, int k, 
     return DM_OK;
 }
 constexpr int MAX_K = 1 << 24;       // values of a row: 32-bit offsets inside a row
-constexpr long MAX_GRID = 0x7fffffffL;
+constexpr long MAX_ROWS = 1L << 40;  // products of rows and groups stay inside 64 bits
+constexpr long MAX_GROUPS = (1L << 32) - 1024;  // of eight values, a thread each at least: a launch holds fewer than 2^32 threads
 Groups groups_of(long rows, int k) {
     Groups n;
     n.gpr = mx_padded(k) / 8;
@@ -320,12 +329,12 @@ int unroll_of(long total) { return total >= 2048L * THREADS * 4 ? 4 : 1; }
 
 extern "C" int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dtype, int fmt, unsigned char* codes, long ldc,
                               unsigned char* scales, long lds, hipStream_t stream) {
-    if (rows < 0 || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
+    if (rows < 0 || rows > MAX_ROWS || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
     if (rows == 0) return DM_OK;
     if (!x || ldx < k) return DM_ERR_ARG;
     if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
     const Groups n = groups_of(rows, k);
-    if (n.total > MAX_GRID * THREADS) return DM_ERR_ARG;
+    if (n.total / unroll_of(n.total) > MAX_GROUPS) return DM_ERR_ARG;
     const int unroll = unroll_of(n.total);
     const dim3 grid((unsigned)((n.total + THREADS * unroll - 1) / (THREADS * unroll)));
 #define DM_MX_Q(T, F)                                                                                                                   \
@@ -339,12 +348,12 @@ extern "C" int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dty
 
 extern "C" int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsigned char* scales, long lds, long rows, int k, int fmt,
                                 void* y, long ldy, int dtype, hipStream_t stream) {
-    if (rows < 0 || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
+    if (rows < 0 || rows > MAX_ROWS || k < 1 || k > MAX_K || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return DM_ERR_ARG;
     if (rows == 0) return DM_OK;
     if (!y || ldy < k) return DM_ERR_ARG;
     if (const int rc = mx_layout(codes, ldc, scales, lds, k, fmt)) return rc;
     const Groups n = groups_of(rows, k);
-    if (n.total > MAX_GRID * THREADS) return DM_ERR_ARG;
+    if (n.total / unroll_of(n.total) > MAX_GROUPS) return DM_ERR_ARG;
     const int unroll = unroll_of(n.total);
     const dim3 grid((unsigned)((n.total + THREADS * unroll - 1) / (THREADS * unroll)));
 #define DM_MX_D(T, F)                                                                                                                     \
@@ -357,12 +366,12 @@ extern "C" int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsi
 }
 
 extern "C" int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream) {
-    if (!d || d->rows < 0 || d->c < 1 || d->c > MAX_K || !dtype_ok(d->dtype) || (d->kind != DM_NORM_RMS && d->kind != DM_NORM_LAYER) ||
+    if (!d || d->rows < 0 || d->rows > MAX_ROWS || d->c < 1 || d->c > MAX_K || !dtype_ok(d->dtype) || (d->kind != DM_NORM_RMS && d->kind != DM_NORM_LAYER) ||
         (d->out_fmt != 0 && !mx_fmt_ok(d->out_fmt)))
         return DM_ERR_ARG;
     if (d->rows == 0) return DM_OK;
     if (!d->x || !d->gamma || !d->y || (d->r == nullptr) != (d->h == nullptr)) return DM_ERR_ARG;
-    if (d->ldx < d->c || (d->r && (d->ldr < d->c || d->ldh < d->c)) || d->rows > MAX_GRID) return DM_ERR_ARG;
+    if (d->ldx < d->c || (d->r && (d->ldr < d->c || d->ldh < d->c))) return DM_ERR_ARG;
     if (d->out_fmt) {
         if (const int rc = mx_layout(d->y, d->ldy, d->y_scales, d->ldys, d->c, d->out_fmt)) return rc;
     } else if (d->ldy < d->c) {

@@ -76,11 +76,11 @@ template <int F> __device__ __forceinline__ void decode_block(const typename MxF
     }
 }
 // GELU(erf) = x Phi(x) for results of 16 bits and fewer: Phi(x) - 1/2 as x times a polynomial of degree 8 in x^2, fitted to
-// minimise the largest error on |x| <= 4.3 and held there beyond (off by at most 1.4e-5 |x|, as gelu_erf_fast_f is).  Twelve
-// full-rate instructions; the exponential and the reciprocal of gelu_erf_fast_f cost four times one each, and 65536 x 2560 x
+// minimise the largest error on |x| <= 4.3 (off by at most 1.4e-5 |x|, as gelu_erf_fast_f is) and held beyond 4.2989, where it
+// passes 1/2: large |x| give x, or 0 to 1e-10 |x|.  Twelve full-rate instructions; the exponential and the reciprocal of gelu_erf_fast_f cost four times one each, and 65536 x 2560 x
 // 320 with GEGLU is bound by its epilogue's instructions.
 __device__ __forceinline__ float gelu_poly_f(float x) {
-    const float c = __builtin_amdgcn_fmed3f(x, -4.3f, 4.3f), u = c * c;
+    const float c = __builtin_amdgcn_fmed3f(x, -4.2989187f, 4.2989187f), u = c * c;
     float q = 5.1566240860667634e-11f;
     q = fmaf(q, u, -5.032703143115214e-09f);
     q = fmaf(q, u, 2.1680975237359235e-07f);
@@ -92,6 +92,9 @@ __device__ __forceinline__ float gelu_poly_f(float x) {
     q = fmaf(q, u, 0.39889654517173767f);
     return x * fmaf(c, q, 0.5f);
 }
+
+// A launch holds fewer than 2^32 threads.
+inline bool mx_grid_ok(long blocks, int threads) { return blocks * threads < (1L << 32); }
 
 // Launches the split kernel on tiles of 16 fm rows by 16 fn rows of W; fm, fn = 1 x 1, 1 x 2, 1 x 4, 2 x 2, 2 x 4 or 4 x 4 (1 x .. where X is
 // plain rows), fn even for GEGLU, whole MX blocks of columns for an MX result.

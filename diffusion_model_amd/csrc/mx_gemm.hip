@@ -351,14 +351,14 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {
     typedef MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES> G;
     constexpr int LDS = G::LDS;
+    const int bo = p.epi == DM_EPI_GEGLU ? BN / 2 : BN;
+    p.tiles_m = (p.m + BM - 1) / BM;
+    p.tiles_n = (p.n_pad + bo - 1) / bo;
+    if (!mx_grid_ok((long)p.tiles_m * p.tiles_n, 64 * G::WAVES)) return DM_ERR_ARG;
     static DmLdsAttr attr;
     const void* fn = reinterpret_cast<const void*>(&mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES>);
     if (LDS > 64 * 1024)
         if (const int rc = dm_set_lds_attr(fn, attr, LDS)) return rc;
-    const int bo = p.epi == DM_EPI_GEGLU ? BN / 2 : BN;
-    p.tiles_m = (p.m + BM - 1) / BM;
-    p.tiles_n = (p.n_pad + bo - 1) / bo;
-    if ((long)p.tiles_m * p.tiles_n > 0x7fffffffL) return DM_ERR_ARG;
     mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }

@@ -274,13 +274,13 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN> int launch_split(MxArgs p, hipStream_t s) {
     constexpr int LDS = SplitRing<XF, WF, FM, FN>::LDS;
     static_assert(32 * FM * FN <= 64 * SPLIT_WAVES, "one thread per eight columns");
-    static DmLdsAttr attr;
-    if (LDS > 64 * 1024)
-        if (const int rc = dm_set_lds_attr(reinterpret_cast<const void*>(&mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN>), attr, LDS)) return rc;
     const int bo = p.epi == DM_EPI_GEGLU ? FN * 8 : FN * 16;
     p.tiles_m = (p.m + 16 * FM - 1) / (16 * FM);
     p.tiles_n = (p.n_pad + bo - 1) / bo;
-    if ((long)p.tiles_m * p.tiles_n > 0x7fffffffL) return DM_ERR_ARG;
+    if (!mx_grid_ok((long)p.tiles_m * p.tiles_n, 64 * SPLIT_WAVES)) return DM_ERR_ARG;
+    static DmLdsAttr attr;
+    if (LDS > 64 * 1024)
+        if (const int rc = dm_set_lds_attr(reinterpret_cast<const void*>(&mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN>), attr, LDS)) return rc;
     mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * SPLIT_WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }

@@ -145,6 +145,21 @@ def test_c_entry_points_refuse_bad_arguments_without_a_device():
         assert gemm(**kw) == 3, kw
 
 
+def test_c_entry_points_refuse_more_than_a_launch_holds():
+    lib = _lib.lib()
+    p = 1 << 20
+    F, B, M8 = _lib.DM_F32, _lib.DM_BF16, _lib.DM_MXFP8
+    assert lib.dm_mx_quantize(p, 1, 1 << 31, 1, F, M8, p, 128, p, 4, None) == 1  # 2^35 groups of eight values, four to a thread
+    assert lib.dm_mx_quantize(p, 1, 1 << 41, 1, F, M8, p, 128, p, 4, None) == 1
+    assert lib.dm_mx_dequantize(p, 128, p, 4, 1 << 31, 1, M8, p, 1, F, None) == 1
+    norm = _lib.RowNormDesc(x=p, ldx=64, gamma=p, y=p, ldy=64, rows=1 << 41, c=64, dtype=F, kind=_lib.NORM_RMS, eps=1e-6)
+    assert lib.dm_row_norm(C.byref(norm), None) == 1
+    for bits, ld, c_type in ((8, 128, B), (4, 64, F)):
+        gemm = _lib.MxGemmDesc(x=p, ldx=ld, x_scales=p, ld_xs=4, w=p, ldw=ld, w_scales=p, ld_ws=4, x_fmt=bits, w_fmt=bits, m=1 << 30, n=4096, k=128,
+                               c=p, ldc=4096, c_type=c_type, epi=_lib.EPI_PLAIN)
+        assert lib.dm_mx_gemm(C.byref(gemm), None) == 1
+
+
 @pytest.mark.gpu
 def test_python_entry_points_refuse_what_does_not_fit(dev):
     x, w = torch.zeros(4, 64, device=dev), mx.quantize(torch.zeros(6, 64, device=dev))
@@ -470,6 +485,34 @@ def test_linear_extreme_scales(dev, xf, wf, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
+@pytest.mark.parametrize("m", [4, 1100])
+def test_linear_smallest_codes_of_the_smallest_scale(dev, xf, wf, m):
+    """Blocks of scale 2^-127 with values below fp32's and bf16's normal range next to large ones: every sum below is exact in
+    fp32 (64 terms of 2 and 64 of 2^-11, or 64 of 2^-5 and 64 of 2^-8), and one rounding away in bf16."""
+    small = -131 if xf == "mxfp8" else -128
+    x = torch.full((m, 128), 2.0 ** (-127 + EMAX[xf]), device=dev)
+    x[:, ::2] = 2.0 ** small
+    xq, wq = mx.quantize(x, xf), mx.quantize(torch.full((1100, 128), 2.0 ** 120, device=dev), wf)
+    assert torch.equal(mx.dequantize(xq), x)
+    sums = 64 * (2.0 ** (EMAX[xf] - 7) + 2.0 ** (small + 120))
+    assert (mx.linear(xq, wq, out_dtype=torch.float32).double() == sums).all()
+    assert ((mx.linear(xq, wq).double() - sums).abs() <= sums * (2.0 ** -8 + 2.0 ** -13)).all()  # the scaled sums, then bf16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 40, 1100])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_geglu_gates_far_from_zero(dev, m, out):
+    """gelu(-512) is 0 and gelu(512) is 512: the polynomial's ends are held where they pass 0 and 1 to 2^-32."""
+    x, w = torch.ones(m, 128, device=dev), torch.ones(256, 128, device=dev)
+    w[128:] = 4
+    w[192:] = -4
+    y = mx.linear(mx.quantize(x, "mxfp4"), mx.quantize(w, "mxfp4"), activation="geglu", out_dtype=out)
+    assert (y[:, :64] == 65536).all() and (y[:, 64:].abs() <= 65536 * 2.0 ** -32).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("xf", FMTS)
 @pytest.mark.parametrize("m,n,k", [(1, 1280, 1280), (1, 33, 45), (4, 640, 1000), (16, 320, 8192), (40, 64, 320), (600, 128, 256)])
@@ -499,6 +542,54 @@ def test_linear_large_equals_blocks_of_it(dev):
         y, size = product(mx.quantize(x[r:r + 1].to(dev), "mxfp4"), wq, None)
         for got in (whole[r:r + 1], part):
             assert bool(((got.cpu().double() - y).abs() <= (k + 2) * U * size).all())
+
+
+# ---- offsets and grids past 32 bits ---------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """Rows 2^24 bytes apart in buffers of 5 GB and results of 2.6 GB give what the same rows side by side give."""
+    rows, k, ld = 300, 1283, 1 << 24
+    x = rows_like(5, rows, k, torch.bfloat16).to(dev)
+    far = torch.zeros(rows * ld // 2, dtype=torch.bfloat16, device=dev).view(rows, ld // 2)[:, 7:7 + k]
+    far.copy_(x)
+    g = torch.linspace(0.5, 2, k, device=dev)
+    assert torch.equal(mx.rmsnorm(far, g), mx.rmsnorm(x, g))
+    (a, h), (b, i) = mx.layernorm(far, g, residual=far, out_format="mxfp8"), mx.layernorm(x, g, residual=x, out_format="mxfp8")
+    assert torch.equal(h, i) and torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    a, b = mx.quantize(far, "mxfp8"), mx.quantize(x, "mxfp8")
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    few = mx.quantize(x[:4], "mxfp4")
+    assert torch.equal(mx.linear(far[-16:], few), mx.linear(x[-16:], few))  # plain rows
+    del far
+    buf = torch.zeros(rows * ld, dtype=torch.uint8, device=dev).view(rows, ld)
+    buf[:, :b.codes.shape[1]], buf[:, 4096:4096 + b.scales.shape[1]] = b.codes, b.scales
+    wide = mx.MXTensor(buf[:, :b.codes.shape[1]], buf[:, 4096:4096 + b.scales.shape[1]], k, "mxfp8")
+    assert torch.equal(mx.dequantize(wide), mx.dequantize(b))
+    w = mx.quantize(rows_like(6, 1000, k, wide=False).to(dev), "mxfp4")
+    for out in DTYPES:
+        assert torch.equal(mx.linear(wide, w, out_dtype=out), mx.linear(b, w, out_dtype=out))  # as the left operand: tiles
+        assert torch.equal(mx.linear(w, wide, out_dtype=out), mx.linear(w, b, out_dtype=out))  # as the right one
+        assert torch.equal(mx.linear(few, wide, out_dtype=out), mx.linear(few, b, out_dtype=out))  # and with few rows
+    del buf, wide
+    m, n, k = 65600, 20000, 96
+    xq, wq = mx.quantize(rows_like(7, m, k, wide=False).to(dev), "mxfp8"), mx.quantize(rows_like(8, n, k, wide=False).to(dev), "mxfp4")
+    tail = mx.MXTensor(xq.codes[-700:], xq.scales[-700:], k, "mxfp8")
+    for kw in (dict(), dict(out_dtype=torch.float32)):
+        assert torch.equal(mx.linear(xq, wq, **kw)[-700:], mx.linear(tail, wq, **kw))
+
+
+@pytest.mark.gpu
+def test_row_norm_of_more_rows_than_a_launch_holds(dev):
+    """2^23 blocks of a row each per launch: the rows before, at and behind the seam, and the last ones."""
+    rows, c = (1 << 23) + 1000, 1027
+    x = torch.empty(rows, c, dtype=torch.bfloat16, device=dev)
+    parts = [slice(0, 300), slice((1 << 23) - 300, (1 << 23) + 300), slice(rows - 300, rows)]
+    for i, part in enumerate(parts):
+        x[part] = rows_like(i, x[part].shape[0], c, torch.bfloat16).to(dev)
+    g, b = torch.linspace(0.5, 2, c, device=dev), torch.linspace(-1, 1, c, device=dev)
+    y = mx.layernorm(x, g, b)
+    for part in parts:
+        assert torch.equal(y[part], mx.layernorm(x[part], g, b))
 
 
 # ---- together, streams, graphs --------------------------------------------------------------------------------------
