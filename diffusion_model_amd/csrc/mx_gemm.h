@@ -47,13 +47,16 @@ __device__ __forceinline__ void to_lds4(const unsigned char* src, unsigned char*
 }
 
 // A k-tile of a row in LDS: 128 values in 128 (e4m3) or 64 (e2m1) bytes, as 16-byte chunks that the XOR below spreads over the
-// banks: any eight consecutive rows occupy eight different 16-byte columns of a 128-byte line.  Requests fill LDS lane by lane, so
-// it is the chunk they fetch that is permuted.
-template <int F> __device__ __forceinline__ int swizzle(int row, int chunk) {
-    return F == 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
+// banks.  A 16-byte read takes four passes of 16 lanes, 0-3, 12-15, 20-27 of each 32 and then the others, and has no conflict when a
+// pass's chunks fill 256 bytes.  A fragment of 32 rows has one chunk number in a pass, one of 16 rows has two that differ in their
+// last bit.  (Counted at 8192^3, 4 bits: with the second form in both, 60 % of the LDS' cycles were conflicts.)
+// Requests fill LDS lane by lane, so it is the chunk they fetch that is permuted.
+template <int F, int ROWS> __device__ __forceinline__ int swizzle(int row, int chunk) {
+    if constexpr (ROWS == 32) return F == 8 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3);
+    else return F == 8 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
 }
-template <int F> __device__ __forceinline__ i32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
-    return *reinterpret_cast<const i32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F>(row, chunk) * 16);
+template <int F, int ROWS> __device__ __forceinline__ i32x4 lds_chunk(const unsigned char* base, int row, int chunk) {
+    return *reinterpret_cast<const i32x4*>(base + row * mx_bytes(F, MX_PAD) + swizzle<F, ROWS>(row, chunk) * 16);
 }
 // A block's 32 values as bf16 with the scale applied (exact: at most four significant bits), in four groups of eight.
 template <int F> __device__ __forceinline__ void decode_block(const typename MxFragment<F>::type& c, float scale, u32x4* out) {

@@ -16,11 +16,11 @@ namespace {
 // EXACT: both formats as the plain block 2 g + j, for products in bf16.
 template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type lds_fragment(const unsigned char* base, int row, int g, int j) {
     if constexpr (F == 8) {
-        const i32x4 lo = lds_chunk<8>(base, row, EXACT ? 2 * (2 * g + j) : 2 * j + g);
-        const i32x4 hi = lds_chunk<8>(base, row, EXACT ? 2 * (2 * g + j) + 1 : 2 * (2 + j) + g);
+        const i32x4 lo = lds_chunk<8, 32>(base, row, EXACT ? 2 * (2 * g + j) : 2 * j + g);
+        const i32x4 hi = lds_chunk<8, 32>(base, row, EXACT ? 2 * (2 * g + j) + 1 : 2 * (2 + j) + g);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-        return lds_chunk<4>(base, row, 2 * g + j);
+        return lds_chunk<4, 32>(base, row, 2 * g + j);
     }
 }
 // Half J of a k-tile: one X fragment with every W fragment.
@@ -186,12 +186,12 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
 #pragma unroll
     for (int i = 0; i < G::PX; ++i) {
         const int row = (wave + i * G::WAVES) * (1024 / G::XB) + lane / (G::XB / 16), pos = lane % (G::XB / 16);
-        xo[i] = (uint32_t)min(row, rows_left) * (uint32_t)p.ldx + swizzle<XF>(row, pos) * 16;
+        xo[i] = (uint32_t)min(row, rows_left) * (uint32_t)p.ldx + swizzle<XF, 32>(row, pos) * 16;
     }
 #pragma unroll
     for (int i = 0; i < G::PW; ++i) {
         const int row = (wave + i * G::WAVES) * (1024 / G::WB) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
-        wo[i] = (uint32_t)w_col(row) * (uint32_t)p.ldw + swizzle<WF>(row, pos) * 16;
+        wo[i] = (uint32_t)w_col(row) * (uint32_t)p.ldw + swizzle<WF, 32>(row, pos) * 16;
     }
     // scalar base + 32-bit lane offset in every request: hidden from the optimiser, which would make each a 64-bit address of its
     // own, carried and advanced in two more registers
@@ -210,7 +210,8 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     };
 
     // quarter q = 4 group + c: rows c (BM + BN) / 4 .. of the group's buffer [row][16 bytes], 16 rows of X or of W per wave and four
-    // lanes per row (waves past the quarter's end repeat others' rows).  Computed without a branch or an indexed register: the
+    // lanes per row (waves past the quarter's end repeat others' rows).  Word w of row r lies at w ^ (r / 8 mod 4): the same
+    // word of 32 rows fills the 32 banks then (4 passes of 8 rows without).  Computed without a branch or an indexed register: the
     // loop below is one block.
     unsigned char* const scales = smem + STAGES * G::STAGE;
     constexpr int QUARTER = (BM + BN) / 4;
@@ -227,7 +228,7 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
         const uint64_t wsrc = wscales + (gate_scales & (0 - (uint64_t)is_gate));
         const uint64_t src = xscales ^ ((xscales ^ wsrc) & ((uint64_t)of_w << 32 | of_w));
         const uint32_t xrow = min(row, rows_left), wrow = w_col(row - BM);
-        const uint32_t at = 4 * min((quarter & ~3) + (lane & 3), last_kt);  // quarters behind the last k-tile repeat it, unread
+        const uint32_t at = 4 * min((quarter & ~3) + ((lane & 3) ^ ((row >> 3) & 3)), last_kt);  // quarters behind the last k-tile repeat it, unread
         const uint32_t off = (xrow ^ ((xrow ^ wrow) & of_w)) * (ld_xs ^ ((ld_xs ^ ld_ws) & of_w)) + at;
         to_lds4((const unsigned char*)src + off, scales + fill * G::GROUP + row0 * 16);
         if ((++quarter & 3) == 0) fill = fill + 1 == G::GROUPS ? 0 : fill + 1;
@@ -270,7 +271,7 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     };
     int next = 0, drain = 0;  // k-tile whose scales are read next and its group's buffer
     auto read_scales = [&]() {
-        const unsigned char* sb = scales + drain * G::GROUP + (next & 3) * 4 + 2 * g;
+        const unsigned char* sb = scales + drain * G::GROUP + ((next & 3) ^ (fr >> 3)) * 4 + 2 * g;
 #pragma unroll
         for (int i = 0; i < FM; ++i) sx_next[i] = *reinterpret_cast<const uint16_t*>(sb + (xrow + i * 32) * 16);
 #pragma unroll

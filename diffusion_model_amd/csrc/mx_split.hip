@@ -29,11 +29,11 @@ template <typename T, int N> __device__ __forceinline__ void load_values(const T
 // EXACT: block g; e4m3: 16 values from 16 g (registers 0-3) and from 64 + 16 g on.  Its scale operand is that of block g either way.
 template <int F, bool EXACT> __device__ __forceinline__ typename MxFragment<F>::type lds_fragment16(const unsigned char* base, int row, int g) {
     if constexpr (F == 8) {
-        const i32x4 lo = lds_chunk<8>(base, row, EXACT ? 2 * g : g);
-        const i32x4 hi = lds_chunk<8>(base, row, EXACT ? 2 * g + 1 : 4 + g);
+        const i32x4 lo = lds_chunk<8, 16>(base, row, EXACT ? 2 * g : g);
+        const i32x4 hi = lds_chunk<8, 16>(base, row, EXACT ? 2 * g + 1 : 4 + g);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-        return lds_chunk<4>(base, row, g);
+        return lds_chunk<4, 16>(base, row, g);
     }
 }
 // One k-tile of 16 plain rows -> codes [16][k-tile] and scales (byte `word` * 4 + block of [16][16]) in LDS: lane (row, block)
@@ -52,7 +52,7 @@ __device__ __forceinline__ void quantize_tile16(const T* row, int k, int kt, int
     }
 #pragma unroll
     for (int c = 0; c < MxCodes<F>::W; ++c)
-        *reinterpret_cast<u32x4*>(codes + r * mx_bytes(F, MX_PAD) + swizzle<F>(r, block * MxCodes<F>::W + c) * 16) = u32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
+        *reinterpret_cast<u32x4*>(codes + r * mx_bytes(F, MX_PAD) + swizzle<F, 16>(r, block * MxCodes<F>::W + c) * 16) = u32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
     scales[r * 16 + word * 4 + block] = (unsigned char)byte;
 }
 template <int XF, int WF, bool EXACT>
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 #pragma unroll
             for (int e = 0; e < G::XN; ++e) {
                 const int r = e * (16 / G::XN) + lane / (G::XB / 16), pos = lane % (G::XB / 16);
-                xp[i][e] = p.x + x_row(i * 16 + r) * p.ldx + swizzle<XF>(r, pos) * 16;
+                xp[i][e] = p.x + x_row(i * 16 + r) * p.ldx + swizzle<XF, 16>(r, pos) * 16;
             }
             xsp[i] = p.xs + x_row(i * 16 + (lane >> 2)) * p.ld_xs;
         } else {
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
 #pragma unroll
         for (int e = 0; e < G::WN; ++e) {
             const int r = e * (16 / G::WN) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
-            wp[j][e] = p.w + w_row(j, r) * p.ldw + swizzle<WF>(r, pos) * 16;
+            wp[j][e] = p.w + w_row(j, r) * p.ldw + swizzle<WF, 16>(r, pos) * 16;
         }
         wsp[j] = p.ws + w_row(j, lane >> 2) * p.ld_ws;
     }
