@@ -180,7 +180,7 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     uint32_t xo[G::PX], wo[G::PW];
     auto w_col = [&](int rho) {  // column of the tile behind LDS row rho
         const int f = rho >> 5, i = rho & 31;
-        return min((geglu ? f >> 1 : f) * 32 + 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3), cols_left);
+        return (geglu ? f >> 1 : f) * 32 + 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
     };
     auto gate = [&](int rho) { return geglu && ((rho >> 5) & 1); };
 #pragma unroll
@@ -191,46 +191,53 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
 #pragma unroll
     for (int i = 0; i < G::PW; ++i) {
         const int row = (wave + i * G::WAVES) * (1024 / G::WB) + lane / (G::WB / 16), pos = lane % (G::WB / 16);
-        wo[i] = (uint32_t)w_col(row) * (uint32_t)p.ldw + swizzle<WF, 32>(row, pos) * 16;
+        wo[i] = (uint32_t)min(w_col(row), cols_left) * (uint32_t)p.ldw + swizzle<WF, 32>(row, pos) * 16;
     }
     // scalar base + 32-bit lane offset in every request: hidden from the optimiser, which would make each a 64-bit address of its
     // own, carried and advanced in two more registers
     auto lane_offset = [](uint32_t o) { asm volatile("" : "+v"(o)); return o; };
-    auto request = [&](int stage) {
+    // requests [from, to) of a k-tile's; the last one moves the sources on
+    constexpr int REQUESTS = G::PX + G::PW;
+    auto request = [&](int stage, int from, int to) {
         unsigned char* base = smem + stage * G::STAGE;
 #pragma unroll
-        for (int i = 0; i < G::PX; ++i) to_lds16(xbase + lane_offset(xo[i]), base + (wave + i * G::WAVES) * 1024);
+        for (int i = 0; i < G::PX; ++i)
+            if (i >= from && i < to) to_lds16(xbase + lane_offset(xo[i]), base + (wave + i * G::WAVES) * 1024);
 #pragma unroll
         for (int i = 0; i < G::PW; ++i) {
             const int slot = wave + i * G::WAVES;
-            to_lds16(wbase + (gate(slot * (1024 / G::WB)) ? gate_bytes : 0) + lane_offset(wo[i]), base + BM * G::XB + slot * 1024);
+            if (G::PX + i >= from && G::PX + i < to) to_lds16(wbase + (gate(slot * (1024 / G::WB)) ? gate_bytes : 0) + lane_offset(wo[i]), base + BM * G::XB + slot * 1024);
         }
-        xbase += G::XB;
-        wbase += G::WB;
+        if (to == REQUESTS) {
+            xbase += G::XB;
+            wbase += G::WB;
+        }
     };
 
-    // quarter q = 4 group + c: rows c (BM + BN) / 4 .. of the group's buffer [row][16 bytes], 16 rows of X or of W per wave and four
-    // lanes per row (waves past the quarter's end repeat others' rows).  Word w of row r lies at w ^ (r / 8 mod 4): the same
-    // word of 32 rows fills the 32 banks then (4 passes of 8 rows without).  Computed without a branch or an indexed register: the
-    // loop below is one block.
+    // quarter q = 4 group + c: of every wave's 64 rows of X or of W those that are c modulo 4, four lanes per row (waves past the
+    // last rows repeat others').  So a lane's row moves on by one with c, within its 32-row fragment and in W's permuted order as
+    // well, and one address per lane does for all four.  The rows lie in the group's buffer as they come, [row / 64][c][row / 4]
+    // [16 bytes], word w of a row at w ^ c: the same word of 32 rows fills the 32 banks then (with the words in order: 4 passes).
+    // Computed without a branch or an indexed register: the loop below is one block.
     unsigned char* const scales = smem + STAGES * G::STAGE;
-    constexpr int QUARTER = (BM + BN) / 4;
-    const int qwave = wave % (QUARTER / 16);
-    const uint64_t xscales = (uint64_t)(p.xs + (long)m0 * p.ld_xs), wscales = (uint64_t)(p.ws + (long)first * p.ld_ws);
-    const uint64_t gate_scales = geglu ? (uint64_t)(p.n_out * p.ld_ws) : 0;
-    const uint32_t ld_xs = (uint32_t)p.ld_xs, ld_ws = (uint32_t)p.ld_ws;
+    const int taker = wave % ((BM + BN) / 64);
+    const bool take_x = taker * 64 < BM;
+    const uint32_t take_ld = (uint32_t)(take_x ? p.ld_xs : p.ld_ws);
+    const unsigned char* take;
+    uint32_t take_span;  // bytes to the last row that exists
+    {
+        const int row0 = taker * 64 + (lane & ~3), left = take_x ? rows_left : cols_left;
+        const int row = min(take_x ? row0 : w_col(row0 - BM), left);
+        take = take_x ? p.xs + m0 * p.ld_xs : p.ws + (first + (gate(row0 - BM) ? p.n_out : 0)) * p.ld_ws;
+        take += row * (long)take_ld;
+        take_span = (uint32_t)(left - row) * take_ld;
+    }
     int quarter = 0, fill = 0;  // next quarter to request and its group's buffer
     const int last_kt = p.nkt - 1;
     auto request_scales = [&]() {
-        const int row0 = (quarter & 3) * QUARTER + qwave * 16, row = row0 + (lane >> 2);
-        const uint32_t of_w = (uint32_t)((BM - 1 - row0) >> 31);  // all ones or zero, as the whole 16 rows are
-        const uint32_t is_gate = ((uint32_t)(row0 - BM) >> 5) & 1;
-        const uint64_t wsrc = wscales + (gate_scales & (0 - (uint64_t)is_gate));
-        const uint64_t src = xscales ^ ((xscales ^ wsrc) & ((uint64_t)of_w << 32 | of_w));
-        const uint32_t xrow = min(row, rows_left), wrow = w_col(row - BM);
-        const uint32_t at = 4 * min((quarter & ~3) + ((lane & 3) ^ ((row >> 3) & 3)), last_kt);  // quarters behind the last k-tile repeat it, unread
-        const uint32_t off = (xrow ^ ((xrow ^ wrow) & of_w)) * (ld_xs ^ ((ld_xs ^ ld_ws) & of_w)) + at;
-        to_lds4((const unsigned char*)src + off, scales + fill * G::GROUP + row0 * 16);
+        const int c = quarter & 3;
+        const uint32_t at = 4 * min((quarter & ~3) + ((lane & 3) ^ c), last_kt);  // quarters behind the last k-tile repeat it, unread
+        to_lds4(take + min(c * take_ld, take_span) + at, scales + fill * G::GROUP + taker * 1024 + c * 256);
         if ((++quarter & 3) == 0) fill = fill + 1 == G::GROUPS ? 0 : fill + 1;
     };
 
@@ -259,7 +266,8 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     // ---- k loop.  A k-tile is two halves of FM x FN matrix instructions.  X fragment i of the next half is read from LDS as
     // soon as the instructions on X fragment i of this one have been issued; W fragments, which all of them use, have two sets.
     // The wait and the barrier for the next k-tile stand behind the first instructions of the second half: every wave has read
-    // all of this k-tile by then, so its stage is refilled at once, and the matrix pipe has work meanwhile.
+    // all of this k-tile by then, so its stage is refilled, a few requests behind each row of instructions (all at once they
+    // cost 8192^3 2 to 4 %: both waves of a SIMD issue them at the same time, and the matrix pipe waits).
     typename MxFragment<XF>::type x[FM];
     typename MxFragment<WF>::type w[2][FN];
     int sx[FM], sw[FN], sx_next[FM], sw_next[FN];
@@ -271,29 +279,28 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     };
     int next = 0, drain = 0;  // k-tile whose scales are read next and its group's buffer
     auto read_scales = [&]() {
-        const unsigned char* sb = scales + drain * G::GROUP + ((next & 3) ^ (fr >> 3)) * 4 + 2 * g;
+        const unsigned char* sb = scales + drain * G::GROUP + (fr & 3) * 256 + (fr >> 2) * 16 + ((next ^ fr) & 3) * 4 + 2 * g;
+        auto fragment = [&](int f) { return *reinterpret_cast<const uint16_t*>(sb + (f >> 1) * 1024 + (f & 1) * 128); };
 #pragma unroll
-        for (int i = 0; i < FM; ++i) sx_next[i] = *reinterpret_cast<const uint16_t*>(sb + (xrow + i * 32) * 16);
+        for (int i = 0; i < FM; ++i) sx_next[i] = fragment(wm * FM + i);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sw_next[j] = *reinterpret_cast<const uint16_t*>(sb + (BM + wrow + j * 32) * 16);
+        for (int j = 0; j < FN; ++j) sw_next[j] = fragment(BM / 32 + wn * FN + j);
         if ((++next & 3) == 0) drain = drain + 1 == G::GROUPS ? 0 : drain + 1;
     };
 
     for (int q = 0; q < STAGES + 3; ++q) request_scales();
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
-        if (s < p.nkt) request(s);
+        if (s < p.nkt) request(s, 0, REQUESTS);
     wait_young<G::LOADS - 1, STAGES - 1>(p.nkt - 1);
     __builtin_amdgcn_s_barrier();
     read_scales();
     read_w(0, 0);
 #pragma unroll
     for (int i = 0; i < FM; ++i) read_x(0, 0, i);
-    constexpr int BARRIER_AT = FM >= 4 ? 1 : 0;
     int stage = 0;
     // LEFT: k-tiles behind this one that have been requested, STAGES - 1 at most; MORE: one more is requested into this one's
-    // stage.  Both are constants and the body has no branch, so the order below is the order of issue.  (Requests spread
-    // between the matrix instructions instead of issued together: no difference at 8192^3, and spills for 8-bit operands.)
+    // stage.  Both are constants and the body has no branch, so the order below is the order of issue.
     auto k_tile = [&](auto left, auto more) {
         constexpr int LEFT = decltype(left)::value;
         constexpr bool MORE = decltype(more)::value;
@@ -314,20 +321,18 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
         for (int i = 0; i < FM; ++i) {
             mma_row<XF, WF, EXACT, 1>(acc[i], x[i], w[1], sx[i], sw);
             if constexpr (LEFT > 0) {
-                if (i == BARRIER_AT) {
+                if (i == 0) {
                     __builtin_amdgcn_sched_barrier(0);
                     wait_vm<(LEFT - 1) * (G::LOADS - 1)>();  // requests of scales among the younger ones only make it wait for more
                     __builtin_amdgcn_s_barrier();
-                    if constexpr (MORE) {
-                        request_scales();
-                        request(here);
-                    }
                     read_scales();
                     read_w(stage, 0);
-#pragma unroll
-                    for (int e = 0; e < BARRIER_AT; ++e) read_x(stage, 0, e);
                 }
-                if (i >= BARRIER_AT) read_x(stage, 0, i);
+                read_x(stage, 0, i);
+                if constexpr (MORE) {
+                    request(here, i * REQUESTS / FM, (i + 1) * REQUESTS / FM);
+                    if (i == FM - 1) request_scales();
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
