@@ -8,7 +8,7 @@
 
 // 16 bytes at any element's address.  Global memory takes unaligned vector accesses, so rows of odd length cost an extra cache
 // line here and there instead of an instruction per value (1001 x 1283 x 1024 with an fp32 result: 18.7 us with scalar stores,
-// x us so).
+// 13 so).
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 __device__ __forceinline__ u32x4 load16_any(const void* p) { return *static_cast<const u32x4_any*>(p); }
 __device__ __forceinline__ void store16_any(void* p, const u32x4& v) { *static_cast<u32x4_any*>(p) = v; }

@@ -33,6 +33,8 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int left, con
 // ---- quantise / dequantise ------------------------------------------------------------------------------------------
 // A lane holds eight values, a quad the 32 of a block.  `gpr` = groups of eight per padded row (a multiple of 16), so a
 // quad never straddles rows; a block sweeps UNROLL x 256 consecutive groups with all its loads ahead of the arithmetic.
+// Bound by HBM: 65536 x 1280 bf16 to 4 bits 50 us (212 MB, 4.2 TB/s; a large copy reaches 5.1 here), back 32 us (6.6 TB/s, what was
+// just written is still cached); 1003 x 1283 fp32 3.3 us, of which 2.5 are the launch.
 struct Groups {
     int gpr;
     uint32_t magic;  // ceil(2^32 / gpr)
@@ -188,7 +190,10 @@ __device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, 
 }
 
 // The row stays in registers: TPR threads of NV groups of eight values, so x and the residual are read once, and the layer
-// norm's variance is a second sum over registers, not a difference of moments.
+// norm's variance is a second sum over registers, not a difference of moments.  Bound by HBM: 16384 x 8192 bf16 with residual to
+// e4m3 190 us (944 MB, 5.0 TB/s; a large copy reaches 5.1); short ones by the chain load - sum - store: 1 x 1280 2.8 us, 1024 x
+// 1280 fp32 6 us (21 MB).  A wave per row up to 1024 values needs no barrier; longer rows are spread over four, so that no
+// lane has more than 64.
 template <typename T, int OUT, int TPR, int NV>
 __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
     __shared__ float red[TPR / 64];

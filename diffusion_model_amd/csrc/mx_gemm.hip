@@ -368,14 +368,15 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }
-// Which tile: measured over m = 1024 .. 65536, n = 1280 .. 5120, k = 320, 1280, 5120 (e4m3 x e2m1, bf16 result) and at 8192^3.
-//   256 x 256  one block per CU.  Where its rounds over the 256 CUs are full and k is long: 8192^3 in 313 us against 381 for
-//              the next (4 bits), 437 against 459 (e4m3 x e2m1); 65536 x 2560 x 1280: 259 against 254
+// Which tile, by measurement on a warm card (e4m3 x e2m1 and a bf16 result where nothing else is said):
+//   256 x 256  one block per CU.  Where its rounds over the 256 CUs are full and k is long: 8192^3 in 289 us against 358 for
+//              the next (4 bits), 400 against 437 (e4m3 x e2m1); 16384 x 5120 x 5120: 351 against 360
 //   128 x 256  two blocks per CU, so that one's epilogue runs beside the other's k loop; W in 4 bits only, whose four
-//              fragments per wave fit the 128 registers that leaves (16384 x 5120 x 320: 61 us against 68 for 256 x 256 and 79 for
-//              128 x 128; x 1280: 122, 129, 138)
-//   128 x 128  two blocks per CU, once there are enough of them, or half as many for a long k
-//   64 x 64    the rest (1024 x 5120 x 1280: 13.9 us against 14.2; 1024 x 1280 x 5120: 22.6 against 28.1)
+//              fragments per wave fit the 128 registers that leaves (16384 x 5120 x 320: 54 us against 57 for 256 x 256 and 56 for
+//              128 x 128; 65536 x 2560 x 320 with GEGLU: 94, 96, 106; 65536 x 2560 x 1280 to bf16: 241, 240)
+//   128 x 128  two blocks per CU, once there is one for each (4096 x 1280 x 1280: 12.2 us against 12.9 for 64 x 64; x 5120: 33
+//              against 41)
+//   64 x 64    the rest (1024 x 1280 x 1280: 7.2 us against 7.5; x 5120: 18.6 against 28.2)
 template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_t s) {
     const int wide = p.epi == DM_EPI_GEGLU ? 2 * p.n_pad : p.n_pad;
     auto tiles = [&](int bm, int bn) { return (long)((p.m + bm - 1) / bm) * ((wide + bn - 1) / bn); };
@@ -386,8 +387,7 @@ template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_
         if constexpr (WF == 4)
             if (tiles(128, 256) >= 512) return launch<XF, WF, EXACT, 128, 256, 32, 128, 2>(p, s);
     }
-    const long t128 = tiles(128, 128);
-    if (t128 >= 512 || (t128 >= 256 && p.nkt >= 20)) return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
+    if (tiles(128, 128) >= 256) return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
     return launch<XF, WF, EXACT, 64, 64, 32, 64, 2>(p, s);
 }
 template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream_t s) {
@@ -396,16 +396,16 @@ template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream
     return launch_fmt<XF, WF, false>(p, s);
 }
 // The split kernel's tile: the smallest that needs at most one block per CU, since blocks read their operands anew
-// (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.1 in 200, the 64 x 64 tile 17; 512 x 1280 x 5120 with the largest 10.5 against 17.6;
-// 256 x 8192 x 8192 in 512 of those 33 against 36, 1024 x 1280 x 5120 in 320 of them 23 against 22).  The largest is slower than
-// the 64 x 64 tile on a short k (512 x 1280 x 320: 5.2 us against 4.5).  Up to 16 rows a tile of 16 x 64 is taken at any size: W
-// is read once then, and that is all there is to do.
+// (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.4 in 200, the 64 x 64 tile 14.4; 128 x 8192 x 8192 with the largest 17.5 against 31.5;
+// 256 x 8192 x 8192 in 512 of those 32.5 against 32.3, 1024 x 1280 x 5120 in 320 of them 23 against 18.6).  The largest is slower than
+// the 64 x 64 tile on a short k (512 x 1280 x 1280: 6.1 us against 5.8; x 5120: 9.8 against 14.6).  Up to 16 rows a tile of 16 x 64 is
+// taken at any size: W is read once then, and that is all there is to do.
 bool split_tile(const MxArgs& p, int* fm, int* fn) {
     static const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {1, 4}, {2, 4}, {4, 4}};
     const bool geglu = p.epi == DM_EPI_GEGLU, mx = p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4;
     for (const auto& t : shapes) {
         const int cols = geglu ? t[1] * 8 : t[1] * 16;
-        if ((geglu && t[1] % 2) || (mx && cols % MX_BLOCK) || (t[0] > 1 && p.m <= 16) || (t[0] == 4 && p.nkt < 8)) continue;
+        if ((geglu && t[1] % 2) || (mx && cols % MX_BLOCK) || (t[0] > 1 && p.m <= 16) || (t[0] == 4 && p.nkt < 16)) continue;
         const long blocks = (long)((p.m + 16 * t[0] - 1) / (16 * t[0])) * ((p.n_pad + cols - 1) / cols);
         if (blocks <= 256 || (p.m <= 16 && t[1] == 4)) {
             *fm = t[0];

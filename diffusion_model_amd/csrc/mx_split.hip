@@ -9,7 +9,7 @@ namespace {
 // Fragments are not loaded straight to registers: the instruction wants 16 rows in 16 neighbouring lanes, and such a load
 // costs a pass per row and quarter wave (measured 61 cycles for 1 KB; 16 x 8192 x 8192 took 11.2 us so, at 14 bytes per cycle and CU
 // whatever cache held them).  A request with four or eight lanes to a row does not: 7.6 us through LDS, 36 MB at 4.8 TB/s with the
-// launch's 2.5 us in it; 77 x 1280 x 5120 5.0 us against 8.2 (and 17 for the 64 x 64 tile).
+// launch's 2.5 us in it; 77 x 1280 x 5120 5.4 us against 8.2 (and 14.4 for the 64 x 64 tile).
 // x_src: X is an MX matrix, or bf16 / fp32 rows that every block quantises as it reads them, a block of 32 values per lane, to
 // the codes that dm_mx_quantize gives.
 constexpr int SPLIT_WAVES = 8;
