@@ -649,6 +649,38 @@ def test_feed_forward_on_another_stream_and_in_a_graph(dev):
 
 
 @pytest.mark.gpu
+def test_calls_at_once_on_two_streams(dev):
+    """The operators share no memory: two streams that run them at the same time give what each gives alone."""
+    jobs = [ff_inputs(dev, rows, 320) for rows in (16, 700)]
+    wants = [feed_forward(*job) for job in jobs]
+    streams = [torch.cuda.Stream(dev) for _ in jobs]
+    torch.cuda.synchronize()
+    gots = [[], []]
+    for _ in range(20):
+        for stream, job, got in zip(streams, jobs, gots):
+            with torch.cuda.stream(stream):
+                got.append(feed_forward(*job))
+    torch.cuda.synchronize()
+    for want, got in zip(wants, gots):
+        assert all(torch.equal(y, want) for y in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [1, 129, 384, 385])
+def test_linear_few_k_tiles_on_the_largest_tile(dev, k):
+    """One to four k-tiles, fewer than the ring's stages and the scales' groups hold (sums of integers, exact in every kernel)."""
+    gen = torch.Generator(device=dev).manual_seed(k)
+    x = torch.randint(-3, 4, (4096, k), generator=gen, device=dev).float()
+    w = torch.randint(-3, 4, (4090, k), generator=gen, device=dev).float()
+    y = torch.mm(x.double(), w.double().t().contiguous())
+    for xf, wf in PAIRS:
+        xq, wq = mx.quantize(x, xf), mx.quantize(w, wf)
+        assert torch.equal(mx.dequantize(xq), x) and torch.equal(mx.dequantize(wq), w)
+        assert torch.equal(mx.linear(xq, wq, out_dtype=torch.float32).double(), y)
+        assert torch.equal(mx.linear(xq, wq), y.bfloat16())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("xf,wf", PAIRS, ids=["a8w4", "a4w4", "a8w8", "a4w8"])
 @pytest.mark.parametrize("m,n,k", [(4000, 3700, 160), (4000, 3700, 4100), (4200, 4100, 200), (2050, 4200, 1400), (1100, 9000, 40)])
 @pytest.mark.parametrize("activation,out", [(None, torch.bfloat16), ("geglu", "mxfp8"), ("quick_gelu", torch.float32)], ids=["bf16", "geglu-mx8", "gelu-f32"])
