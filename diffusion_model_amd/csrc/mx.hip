@@ -171,11 +171,23 @@ __device__ __forceinline__ void load_affine(const NormArgs& p, int at, float* ga
     load8<float>(p.gamma + at, p.c - at, gamma);
     if (p.beta) load8<float>(p.beta + at, p.c - at, beta);
 }
+// v / sqrt(s), rounded once: the product with the reciprocal is corrected by its remainder.  (The product alone is off by up to
+// 1.5 units, for a whole row at once, and values next to a code's border change sides: 3e-5 of a 16384 x 8192 result in e4m3 against an
+// fp32 division, 4e-6 so.  The launch waits for memory, the three instructions cost it nothing.)
+struct Root {
+    float root, inverse;
+    bool plain;  // no remainder where one of them is 0 or infinite
+    __device__ __forceinline__ explicit Root(float s) : root(sqrtf(s)), inverse(1.f / root), plain(!(inverse > 0.f && inverse < INFINITY)) {}
+    __device__ __forceinline__ float divide(float v) const {
+        const float q = v * inverse;
+        return plain ? q : fmaf(fmaf(-q, root, v), inverse, q);
+    }
+};
 template <typename T, int OUT>
-__device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, float rstd, const float* gamma, const float* beta) {
+__device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, const Root& root, const float* gamma, const float* beta) {
     float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (v[i] - mean) * rstd * gamma[i];
+    for (int i = 0; i < 8; ++i) o[i] = root.divide(v[i] - mean) * gamma[i];
     if (p.beta) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] += beta[i];
@@ -233,12 +245,12 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
             }
         s = row_sum<TPR>(s, red) / p.c;
     }
-    const float rstd = 1.f / sqrtf(s + p.eps);
+    const Root root(s + p.eps);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
         if ((n * TPR + t) * 8 < cp) {
             if constexpr (!EARLY) load_affine(p, (n * TPR + t) * 8, gamma[0], beta[0]);
-            norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, rstd, gamma[EARLY ? n : 0], beta[EARLY ? n : 0]);
+            norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, root, gamma[EARLY ? n : 0], beta[EARLY ? n : 0]);
         }
 }
 
@@ -273,13 +285,13 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
         }
         s = row_sum<THREADS>(s, red) / p.c;
     }
-    const float rstd = 1.f / sqrtf(s + p.eps);
+    const Root root(s + p.eps);
     for (int at = threadIdx.x * 8; at < cp; at += THREADS * 8) {
         float v[8];
         load8<T>(stored + at, p.c - at, v);
         float gamma[8], beta[8];
         load_affine(p, at, gamma, beta);
-        norm_store<T, OUT>(p, row, at, v, mean, rstd, gamma, beta);
+        norm_store<T, OUT>(p, row, at, v, mean, root, gamma, beta);
     }
 }
 
