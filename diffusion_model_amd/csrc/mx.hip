@@ -130,14 +130,16 @@ struct NormArgs {
     long rows, first;  // rows of the matrix; row of the launch's first block
     int c, layer;
     float eps;
+    double inverse;  // 1 / c
 };
 
 // Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.  Inside 16 lanes by DPP (a shuffle
-// through LDS takes an order of magnitude longer, and short rows are bound by this chain).
+// through LDS takes an order of magnitude longer, and short rows are bound by this chain).  Waves are joined in 64 bits, and
+// the mean is taken there: the last additions are the ones whose rounding the whole row would share.
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
 }
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+template <int TPR> __device__ __forceinline__ double row_sum(float v, float* red) {
     v = dpp_add<0xB1>(v);   // quad_perm 1 0 3 2
     v = dpp_add<0x4E>(v);   // quad_perm 2 3 0 1
     v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of eight lanes
@@ -148,9 +150,10 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red)
         __syncthreads();  // the previous sum has been read
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.f;
+        double sum = 0.;
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) v += red[i];
+        for (int i = 0; i < TPR / 64; ++i) sum += red[i];
+        return sum;
     }
     return v;
 }
@@ -172,8 +175,8 @@ __device__ __forceinline__ void load_affine(const NormArgs& p, int at, float* ga
     if (p.beta) load8<float>(p.beta + at, p.c - at, beta);
 }
 // v / sqrt(s), rounded once: the product with the reciprocal is corrected by its remainder.  (The product alone is off by up to
-// 1.5 units, for a whole row at once, and values next to a code's border change sides: 3e-5 of a 16384 x 8192 result in e4m3 against an
-// fp32 division, 4e-6 so.  The launch waits for memory, the three instructions cost it nothing.)
+// 1.5 units, for a whole row at once, and values next to a code's border change sides: a 16384 x 8192 result in e4m3 was
+// 3e-5 from the definition in 64 bits, and is 0 with this and the sum above.  The launch waits for memory, the three instructions cost it nothing.)
 struct Root {
     float root, inverse;
     bool plain;  // no remainder where one of them is 0 or infinite
@@ -231,10 +234,10 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += p.layer ? v[n][i] : v[n][i] * v[n][i];
     }
-    s = row_sum<TPR>(s, red) / p.c;
+    double m = row_sum<TPR>(s, red) * p.inverse;
     float mean = 0.f;
     if (p.layer) {
-        mean = s;
+        mean = (float)m;
         s = 0.f;
 #pragma unroll
         for (int n = 0; n < NV; ++n)
@@ -243,9 +246,9 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
                 const float d = (n * TPR + t) * 8 + i < p.c ? v[n][i] - mean : 0.f;
                 s = fmaf(d, d, s);
             }
-        s = row_sum<TPR>(s, red) / p.c;
+        m = row_sum<TPR>(s, red) * p.inverse;
     }
-    const Root root(s + p.eps);
+    const Root root((float)(m + p.eps));
 #pragma unroll
     for (int n = 0; n < NV; ++n)
         if ((n * TPR + t) * 8 < cp) {
@@ -270,9 +273,9 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += p.layer ? v[i] : v[i] * v[i];
     }
-    s = row_sum<THREADS>(s, red) / p.c;
+    double m = row_sum<THREADS>(s, red) * p.inverse;
     if (p.layer) {
-        mean = s;
+        mean = (float)m;
         s = 0.f;
         for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
             float v[8];
@@ -283,9 +286,9 @@ template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_no
                 s = fmaf(d, d, s);
             }
         }
-        s = row_sum<THREADS>(s, red) / p.c;
+        m = row_sum<THREADS>(s, red) * p.inverse;
     }
-    const Root root(s + p.eps);
+    const Root root((float)(m + p.eps));
     for (int at = threadIdx.x * 8; at < cp; at += THREADS * 8) {
         float v[8];
         load8<T>(stored + at, p.c - at, v);
@@ -398,6 +401,7 @@ extern "C" int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream) {
     p.x = d->x; p.r = d->r; p.h = d->h; p.gamma = d->gamma; p.beta = d->beta; p.y = d->y; p.ys = d->y_scales;
     p.ldx = d->ldx; p.ldr = d->ldr; p.ldh = d->ldh; p.ldy = d->ldy; p.ldys = d->ldys;
     p.rows = d->rows; p.c = d->c; p.layer = d->kind == DM_NORM_LAYER; p.eps = d->eps;
+    p.inverse = 1. / d->c;
 #define DM_NORM(T) \
     (d->out_fmt == 0 ? launch_norm<T, 0>(p, stream) : d->out_fmt == DM_MXFP8 ? launch_norm<T, 8>(p, stream) : launch_norm<T, 4>(p, stream))
     return d->dtype == DM_F32 ? DM_NORM(float) : DM_NORM(bf16_t);

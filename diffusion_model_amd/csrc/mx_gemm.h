@@ -80,8 +80,8 @@ template <int F> __device__ __forceinline__ void decode_block(const typename MxF
 }
 // GELU(erf) = x Phi(x) for results of 16 bits and fewer: Phi(x) - 1/2 as x times a polynomial of degree 8 in x^2, fitted to
 // minimise the largest error on |x| <= 4.3 (off by at most 1.4e-5 |x|, as gelu_erf_fast_f is) and held beyond 4.2989, where it
-// passes 1/2: large |x| give x, or 0 to 1e-10 |x|.  Twelve full-rate instructions; the exponential and the reciprocal of gelu_erf_fast_f cost four times one each, and the epilogue of 65536 x 2560 x
-// 320 with GEGLU is 40 % of its time.
+// passes 1/2: large |x| give x, or 0 to 1e-10 |x|.  Twelve full-rate instructions; the exponential and the reciprocal of
+// gelu_erf_fast_f cost four times one each, and the epilogue of 65536 x 2560 x 320 with GEGLU is 40 % of its time.
 __device__ __forceinline__ float gelu_poly_f(float x) {
     const float c = __builtin_amdgcn_fmed3f(x, -4.2989187f, 4.2989187f), u = c * c;
     float q = 5.1566240860667634e-11f;
