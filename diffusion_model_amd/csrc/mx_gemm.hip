@@ -224,13 +224,13 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     const bool take_x = taker * 64 < BM;
     const uint32_t take_ld = (uint32_t)(take_x ? p.ld_xs : p.ld_ws);
     const unsigned char* take;
-    uint32_t take_span;  // bytes to the last row that exists
+    uint32_t take_span;  // bytes to the last of the next three rows that exists: below 2^26, whatever the matrix spans
     {
         const int row0 = taker * 64 + (lane & ~3), left = take_x ? rows_left : cols_left;
         const int row = min(take_x ? row0 : w_col(row0 - BM), left);
         take = take_x ? p.xs + m0 * p.ld_xs : p.ws + (first + (gate(row0 - BM) ? p.n_out : 0)) * p.ld_ws;
         take += row * (long)take_ld;
-        take_span = (uint32_t)(left - row) * take_ld;
+        take_span = (uint32_t)min(left - row, 3) * take_ld;
     }
     int quarter = 0, fill = 0;  // next quarter to request and its group's buffer
     const int last_kt = p.nkt - 1;
