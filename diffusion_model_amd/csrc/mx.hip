@@ -133,29 +133,69 @@ struct NormArgs {
     double inverse;  // 1 / c
 };
 
-// Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.  Inside 16 lanes by DPP (a shuffle
-// through LDS takes an order of magnitude longer, and short rows are bound by this chain).  Waves are joined in 64 bits, and
-// the mean is taken there: the last additions are the ones whose rounding the whole row would share.
-template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+// Sum over the TPR threads that share a row, in a fixed order: every one of them gets it.  By DPP and lane swaps (a shuffle
+// through LDS takes an order of magnitude longer, and short rows are bound by this chain).  In 64 bits like the threads' own
+// sums, which hold any square and add equal terms without drifting; fp32 sums cost a constant row of 1000.1 a mean that is off by 11
+// units at 8192 values, and a row of 2^24 values 2.6e-4 of its RMS.
+template <int CTRL> __device__ __forceinline__ double dpp_add(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 o = {(uint32_t)__builtin_amdgcn_mov_dpp((int)w[0], CTRL, 0xF, 0xF, true), (uint32_t)__builtin_amdgcn_mov_dpp((int)w[1], CTRL, 0xF, 0xF, true)};
+    return v + __builtin_bit_cast(double, o);
 }
-template <int TPR> __device__ __forceinline__ double row_sum(float v, float* red) {
+// v plus the other 16 lanes' of 32 (W = 16) or the other half wave's (W = 32): the swap leaves one half's values in the first word
+// of every lane and the other's in the second.
+template <int W> __device__ __forceinline__ double swap_add(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    u32x2 a, b;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto t = W == 16 ? __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false) : __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        a[i] = t[0];
+        b[i] = t[1];
+    }
+    return __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b);
+}
+template <int TPR> __device__ __forceinline__ double row_sum(double v, double* red) {
     v = dpp_add<0xB1>(v);   // quad_perm 1 0 3 2
     v = dpp_add<0x4E>(v);   // quad_perm 2 3 0 1
     v = dpp_add<0x141>(v);  // row_half_mirror: the other quad of eight lanes
     v = dpp_add<0x140>(v);  // row_mirror: the other eight of sixteen
-    v += __shfl_xor(v, 16);
-    v += __shfl_xor(v, 32);
+    v = swap_add<16>(v);
+    v = swap_add<32>(v);
     if constexpr (TPR > 64) {
         __syncthreads();  // the previous sum has been read
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        double sum = 0.;
+        v = red[0];
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) sum += red[i];
-        return sum;
+        for (int i = 1; i < TPR / 64; ++i) v += red[i];
     }
     return v;
+}
+// Eight values on top of a thread's sum for the mean (layer) or the mean square, in two chains.
+__device__ __forceinline__ double add8(double s, const float* v, bool layer) {
+    double a = 0., b = 0.;
+    if (layer) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) { a += v[i]; b += v[i + 1]; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) { a = fma((double)v[i], (double)v[i], a); b = fma((double)v[i + 1], (double)v[i + 1], b); }
+    }
+    return s + (a + b);
+}
+// A mean as two fp32 numbers: v - mean keeps its bits where the row lies far from zero.
+struct Mean {
+    float high = 0.f, low = 0.f;
+    __device__ __forceinline__ Mean() {}
+    __device__ __forceinline__ explicit Mean(double m) : high((float)m), low((float)(m - high)) {}
+    __device__ __forceinline__ float distance(float v) const { return (v - high) - low; }
+};
+// Eight values become their distances from the mean (0 from `left` on), whose squares go on top of a thread's sum.
+__device__ __forceinline__ double add8_squares(double s, float* v, const Mean& mean, int left) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? mean.distance(v[i]) : 0.f;
+    return add8(s, v, false);
 }
 // eight values of h = x + r, rounded to the storage type (the norm is that of the stored row)
 template <typename T> __device__ __forceinline__ void load_h(const NormArgs& p, long row, int at, float* v) {
@@ -175,22 +215,29 @@ __device__ __forceinline__ void load_affine(const NormArgs& p, int at, float* ga
     if (p.beta) load8<float>(p.beta + at, p.c - at, beta);
 }
 // v / sqrt(s), rounded once: the product with the reciprocal is corrected by its remainder.  (The product alone is off by up to
-// 1.5 units, for a whole row at once, and values next to a code's border change sides: a 16384 x 8192 result in e4m3 was
-// 3e-5 from the definition in 64 bits, and is 0 with this and the sum above.  The launch waits for memory, the three instructions cost it nothing.)
+// 1.5 units, for a whole row at once, and values next to a code's border change sides.)  Both sides are scaled by the power of two
+// that brings the root next to 1, so that the steps between stay in fp32's normal range for every s.
 struct Root {
-    float root, inverse;
-    bool plain;  // no remainder where one of them is 0 or infinite
-    __device__ __forceinline__ explicit Root(float s) : root(sqrtf(s)), inverse(1.f / root), plain(!(inverse > 0.f && inverse < INFINITY)) {}
+    float scale, root, inverse;
+    bool plain;  // no remainder where the root is 0, infinite or NaN
+    __device__ __forceinline__ explicit Root(double s) {
+        const int e = ((int)((__builtin_bit_cast(u32x2, s)[1] >> 20) & 2047u) - 1023) >> 1;
+        const int by = -min(max(e, -126), 126);
+        scale = __uint_as_float((uint32_t)(by + 127) << 23);
+        root = sqrtf((float)__builtin_ldexp(s, 2 * by));
+        inverse = 1.f / root;
+        plain = !(inverse > 0.f && inverse < INFINITY);
+    }
     __device__ __forceinline__ float divide(float v) const {
-        const float q = v * inverse;
-        return plain ? q : fmaf(fmaf(-q, root, v), inverse, q);
+        const float u = v * scale, q = u * inverse;
+        return plain ? q : fmaf(fmaf(-q, root, u), inverse, q);
     }
 };
 template <typename T, int OUT>
-__device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, float mean, const Root& root, const float* gamma, const float* beta) {
+__device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, const float* v, const Root& root, const float* gamma, const float* beta) {
     float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = root.divide(v[i] - mean) * gamma[i];
+    for (int i = 0; i < 8; ++i) o[i] = root.divide(v[i]) * gamma[i];
     if (p.beta) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] += beta[i];
@@ -211,7 +258,7 @@ __device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, 
 // lane has more than 64.
 template <typename T, int OUT, int TPR, int NV>
 __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
-    __shared__ float red[TPR / 64];
+    __shared__ double red[TPR / 64];
     const int t = threadIdx.x % TPR;
     const long row = p.first + (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
     if (row >= p.rows) return;  // whole waves; TPR > 64 has one row per block
@@ -226,34 +273,27 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
 #pragma unroll
         for (int n = 0; n < NV; ++n) load_affine(p, (n * TPR + t) * 8, gamma[n], beta[n]);
     }
-    float s = 0.f;
+    double s = 0.;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
         const int at = (n * TPR + t) * 8;
         if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, v[n]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += p.layer ? v[n][i] : v[n][i] * v[n][i];
+        s = add8(s, v[n], p.layer);
     }
     double m = row_sum<TPR>(s, red) * p.inverse;
-    float mean = 0.f;
     if (p.layer) {
-        mean = (float)m;
-        s = 0.f;
+        const Mean mean(m);
+        s = 0.;
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = (n * TPR + t) * 8 + i < p.c ? v[n][i] - mean : 0.f;
-                s = fmaf(d, d, s);
-            }
+        for (int n = 0; n < NV; ++n) s = add8_squares(s, v[n], mean, p.c - (n * TPR + t) * 8);
         m = row_sum<TPR>(s, red) * p.inverse;
     }
-    const Root root((float)(m + p.eps));
+    const Root root(m + p.eps);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
         if ((n * TPR + t) * 8 < cp) {
             if constexpr (!EARLY) load_affine(p, (n * TPR + t) * 8, gamma[0], beta[0]);
-            norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], mean, root, gamma[EARLY ? n : 0], beta[EARLY ? n : 0]);
+            norm_store<T, OUT>(p, row, (n * TPR + t) * 8, v[n], root, gamma[EARLY ? n : 0], beta[EARLY ? n : 0]);
         }
 }
 
@@ -261,40 +301,40 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
 // first are served by the caches.  With a residual they read the stored h (each thread what it wrote itself), so h may be x
 // or the residual itself here as in the kernel above.
 template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_norm_loop_kernel(NormArgs p) {
-    __shared__ float red[THREADS / 64];
+    __shared__ double red[THREADS / 64];
     const long row = p.first + blockIdx.x;
     const int cp = OUT ? mx_padded(p.c) : p.c;
     const T* stored = p.r ? static_cast<const T*>(p.h) + row * p.ldh : static_cast<const T*>(p.x) + row * p.ldx;
-    float s = 0.f, mean = 0.f;
+    double s = 0.;
+    Mean mean;
     for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
         float v[8];
         load_h<T>(p, row, at, v);
         if (p.r) store8<T>(static_cast<T*>(p.h) + row * p.ldh + at, p.c - at, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += p.layer ? v[i] : v[i] * v[i];
+        s = add8(s, v, p.layer);
     }
     double m = row_sum<THREADS>(s, red) * p.inverse;
     if (p.layer) {
-        mean = (float)m;
-        s = 0.f;
+        mean = Mean(m);
+        s = 0.;
         for (int at = threadIdx.x * 8; at < p.c; at += THREADS * 8) {
             float v[8];
             load8<T>(stored + at, p.c - at, v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = at + i < p.c ? v[i] - mean : 0.f;
-                s = fmaf(d, d, s);
-            }
+            s = add8_squares(s, v, mean, p.c - at);
         }
         m = row_sum<THREADS>(s, red) * p.inverse;
     }
-    const Root root((float)(m + p.eps));
+    const Root root(m + p.eps);
     for (int at = threadIdx.x * 8; at < cp; at += THREADS * 8) {
         float v[8];
         load8<T>(stored + at, p.c - at, v);
         float gamma[8], beta[8];
         load_affine(p, at, gamma, beta);
-        norm_store<T, OUT>(p, row, at, v, mean, root, gamma, beta);
+        if (p.layer) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mean.distance(v[i]);
+        }
+        norm_store<T, OUT>(p, row, at, v, root, gamma, beta);
     }
 }
 

@@ -315,7 +315,7 @@ int dm_mx_dequantize(const unsigned char* codes, long ldc, const unsigned char* 
  *   DM_NORM_RMS:   y = h / sqrt(mean(h^2) + eps) * gamma (+ beta)
  *   DM_NORM_LAYER: y = (h - mean(h)) / sqrt(var(h) + eps) * gamma (+ beta)     (blocks.py:137,143,149; clip.py:99,110)
  * y: rows of ldy elements of dtype (out_fmt 0), or an MX matrix of c values per row (out_fmt DM_MXFP8 / DM_MXFP4: y = codes,
- * ldy bytes; y_scales, ldys).  Statistics in fp32.  r and h go together and are rows of dtype; h may be x or r itself, and y may
+ * ldy bytes; y_scales, ldys).  Statistics in fp64.  r and h go together and are rows of dtype; h may be x or r itself, and y may
  * be x when there is no quantisation.  Any row length up to 2^24 and any alignment. */
 #define DM_NORM_RMS 0
 #define DM_NORM_LAYER 1
