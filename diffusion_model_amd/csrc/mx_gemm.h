@@ -78,6 +78,26 @@ template <int F> __device__ __forceinline__ void decode_block(const typename MxF
         }
     }
 }
+// Activations of fp32 results, right to a few units of the result where it is small, too.  An exponential's argument is rounded by
+// up to 2^-24 of itself, the exponential by that times the argument, so what the rounding dropped is multiplied on behind it.  Both begin
+// from the negative side's value, e or Phi(-|x|), which a sum with 1 would have swallowed: 1 + erff loses 2e-4 of the result at a
+// gate of -4, 4 % at -5 and all of it from -5.5 on.  Finite bounds, where the exponential is 0 already, keep infinity - infinity
+// out; the product with x then gives what IEEE arithmetic says.
+__device__ __forceinline__ float quick_gelu_f32(float v) {
+    constexpr float rate = 1.702f, rate_rest = (float)(1.702 - (double)1.702f);
+    const float t = fminf(fabsf(v), 128.f), a = rate * t, rest = fmaf(rate_rest, t, fmaf(rate, t, -a));
+    float e = expf(-a);
+    e = fmaf(-e, rest, e);
+    return v * (v < 0.f ? e : 1.f) / (1.f + e);
+}
+// x Phi(x), Phi(-t) = exp(-t^2 / 2) erfcx(t / sqrt 2) / 2
+__device__ __forceinline__ float gelu_f32(float x) {
+    const float t = fminf(fabsf(x), 20.f), a = t * t, rest = fmaf(t, t, -a);
+    float e = expf(-0.5f * a);
+    e = fmaf(-0.5f * e, rest, e);
+    const float q = 0.5f * e * erfcxf(t * 0.70710678118654752440f);
+    return x * (x < 0.f ? q : 1.f - q);
+}
 // GELU(erf) = x Phi(x) for results of 16 bits and fewer: Phi(x) - 1/2 as x times a polynomial of degree 8 in x^2, fitted to
 // minimise the largest error on |x| <= 4.3 (off by at most 1.4e-5 |x|, as gelu_erf_fast_f is) and held beyond 4.2989, where it
 // passes 1/2: large |x| give x, or 0 to 1e-10 |x|.  Twelve full-rate instructions; the exponential and the reciprocal of

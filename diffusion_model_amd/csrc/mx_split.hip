@@ -263,10 +263,10 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
         float gate[8];
         total(2 * (c8 >> 1) + 1, p.n_out + col, gate);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= p.c_type == DM_F32 ? gelu_erf_f(gate[e]) : gelu_poly_f(gate[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= p.c_type == DM_F32 ? gelu_f32(gate[e]) : gelu_poly_f(gate[e]);
     } else if (p.epi == DM_EPI_QUICKGELU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + __expf(-1.702f * v[e]));
+        for (int e = 0; e < 8; ++e) v[e] = p.c_type == DM_F32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));
     }
     store8(p, m0 + row, col, v, threadIdx.x);
 }
