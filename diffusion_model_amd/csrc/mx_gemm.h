@@ -26,6 +26,12 @@ struct MxArgs {
     int k;                // X as plain rows: values of a row
 };
 
+// Result types of a kernel: fp32 results of e4m3 operands come from the EXACT kernels alone, which give nothing else.
+enum class MxResults { FP32, BF16_MX, ANY };
+constexpr MxResults mx_results(int xf, int wf, bool exact) {
+    return exact ? MxResults::FP32 : xf == 8 || wf == 8 ? MxResults::BF16_MX : MxResults::ANY;
+}
+
 __device__ __forceinline__ i32x8 widen(const i32x8& v) { return v; }
 __device__ __forceinline__ i32x8 widen(const i32x4& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }  // the instruction reads four registers
 // Also waits for this wave's LDS reads: what follows is the barrier behind which other waves refill what they read.

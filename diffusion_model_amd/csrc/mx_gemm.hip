@@ -112,10 +112,16 @@ __device__ __forceinline__ void store_fragments(const MxArgs& p, const f32x16 (&
             store16<CT>(p, row(i), column(j), v, lane, edge);
         }
 }
-template <int EPI, int FM, int FN, typename Row, typename Column>
+// RESULTS: the types that the kernel is launched for (fp32 results of e4m3 operands have kernels of their own)
+template <int EPI, MxResults RESULTS, int FM, int FN, typename Row, typename Column>
 __device__ __forceinline__ void store_typed(const MxArgs& p, const f32x16 (&acc)[FM][FN], Row row, Column column, int lane, bool edge) {
+    if constexpr (RESULTS == MxResults::FP32) {
+        store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
+        return;
+    }
+    if constexpr (RESULTS == MxResults::ANY)
+        if (p.c_type == DM_F32) return store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
     if (p.c_type == DM_BF16) store_fragments<EPI, DM_BF16>(p, acc, row, column, lane, edge);
-    else if (p.c_type == DM_F32) store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
     else if (p.c_type == DM_MXFP8) store_fragments<EPI, DM_MXFP8>(p, acc, row, column, lane, edge);
     else store_fragments<EPI, DM_MXFP4>(p, acc, row, column, lane, edge);
 }
@@ -347,11 +353,12 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     k_tile(std::integral_constant<int, 0>(), std::false_type());
 
     // ---- epilogue: a lane holds row .. + fr and 16 columns per fragment
+    constexpr MxResults RESULTS = mx_results(XF, WF, EXACT);
     const bool edge = col0 + (geglu ? BN / 2 : BN) > p.n_out;
     auto row = [&](int i) { return (long)(m0 + wm * WM + i * 32 + fr); };
-    if (geglu) store_typed<DM_EPI_GEGLU>(p, acc, row, column, lane, edge);
-    else if (p.epi == DM_EPI_QUICKGELU) store_typed<DM_EPI_QUICKGELU>(p, acc, row, column, lane, edge);
-    else store_typed<DM_EPI_PLAIN>(p, acc, row, column, lane, edge);
+    if (geglu) store_typed<DM_EPI_GEGLU, RESULTS>(p, acc, row, column, lane, edge);
+    else if (p.epi == DM_EPI_QUICKGELU) store_typed<DM_EPI_QUICKGELU, RESULTS>(p, acc, row, column, lane, edge);
+    else store_typed<DM_EPI_PLAIN, RESULTS>(p, acc, row, column, lane, edge);
 }
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {

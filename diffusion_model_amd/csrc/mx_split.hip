@@ -68,8 +68,8 @@ __device__ __forceinline__ void mma16(f32x4& acc, const typename MxFragment<XF>:
     }
 }
 // Columns col .. col + 7 of row m; the four lanes of a quad hold the 32 columns of an MX block.
-__device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* v, int lane) {
-    if (p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4) {
+__device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* v, int lane, bool f32) {
+    if (!f32 && (p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4)) {
         if (col >= p.n_pad) return;  // whole quads
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = col + e < p.n_out ? v[e] : 0.f;
@@ -79,7 +79,7 @@ __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* 
         return;
     }
     const int left = p.n_out - col;
-    if (p.c_type == DM_BF16) {
+    if (!f32) {
         bf16_t* dst = static_cast<bf16_t*>(p.c) + m * p.ldc + col;
         float r[8] = {};
         if (p.r) load_values<bf16_t, 8>(static_cast<const bf16_t*>(p.r) + m * p.ldr + col, left, r);
@@ -257,18 +257,20 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
                 for (int e = 0; e < 4; ++e) v[4 * h + e] += t[e];
             }
     };
+    constexpr MxResults RESULTS = mx_results(XF, WF, EXACT);
+    const bool f32 = RESULTS == MxResults::FP32 || (RESULTS == MxResults::ANY && p.c_type == DM_F32);
     float v[8];
     total(geglu ? 2 * (c8 >> 1) : c8 >> 1, col, v);
     if (geglu) {
         float gate[8];
         total(2 * (c8 >> 1) + 1, p.n_out + col, gate);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= p.c_type == DM_F32 ? gelu_f32(gate[e]) : gelu_poly_f(gate[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= f32 ? gelu_f32(gate[e]) : gelu_poly_f(gate[e]);
     } else if (p.epi == DM_EPI_QUICKGELU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = p.c_type == DM_F32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));
+        for (int e = 0; e < 8; ++e) v[e] = f32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));
     }
-    store8(p, m0 + row, col, v, threadIdx.x);
+    store8(p, m0 + row, col, v, threadIdx.x, f32);
 }
 
 template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN> int launch_split(MxArgs p, hipStream_t s) {
