@@ -102,7 +102,7 @@ __device__ __forceinline__ void store_fragments(const MxArgs& p, const f32x16 (&
                 const float o = acc[i][j][e];
                 if constexpr (EPI == DM_EPI_GEGLU) {
                     const float gate = acc[i][j + STEP - 1][e];
-                    v[e] = o * (CT == DM_F32 ? gelu_f32(gate) : gelu_poly_f(gate));
+                    v[e] = o * (CT == DM_F32 ? gelu_f32(gate) : gelu_exp2_f(gate));
                 } else if constexpr (EPI == DM_EPI_QUICKGELU) {
                     v[e] = CT == DM_F32 ? quick_gelu_f32(o) : o / (1.f + __expf(-1.702f * o));
                 } else {

@@ -265,7 +265,7 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
         float gate[8];
         total(2 * (c8 >> 1) + 1, p.n_out + col, gate);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f32 ? gelu_f32(gate[e]) : gelu_poly_f(gate[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= f32 ? gelu_f32(gate[e]) : gelu_exp2_f(gate[e]);
     } else if (p.epi == DM_EPI_QUICKGELU) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = f32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));

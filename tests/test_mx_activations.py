@@ -68,7 +68,16 @@ def test_gelu_gates_in_fp32(dev, m):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [4, 301])
-@pytest.mark.parametrize("out", [torch.float32], ids=["f32"])
+def test_gelu_gates_in_bf16(dev, m):
+    """The type's rounding, and an eighth of it for the gate; a Phi below the smallest normal number may vanish (13 2^-126)."""
+    g = arguments(dev, -13.0, 13.0)
+    got = product_of(dev, m, torch.cat([torch.ones_like(g), g]), activation="geglu")
+    check(got, gelu(g), 2.0 ** -8 + 2.0 ** -11, 2.0 ** -122)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 301])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 def test_gates_that_are_huge_or_not_finite(dev, m, out):
     """g Phi(g) in IEEE arithmetic: g where Phi is 1, 0 where it is 0, NaN for -inf (-inf times 0) and NaN."""
     inf = float("inf")
