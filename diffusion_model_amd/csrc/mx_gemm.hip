@@ -148,7 +148,7 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     static_assert(BM % 64 == 0 && BN % 64 == 0 && WM % 32 == 0 && WN % 32 == 0, "whole requests and fragments");
     static_assert(PX * WAVES * 1024 == BM * XB && PW * WAVES * 1024 == BN * WB && (BM + BN) / 64 <= WAVES, "every wave requests the same");
     static_assert(WN % 64 == 0, "a wave holds both the values and the gates of its columns");
-    static_assert((STAGES - 1) * LOADS <= 63 && (STAGES == 2 || STAGES == 3), "vmcnt counts to 63; the tail of the k loop");
+    static_assert((STAGES - 1) * LOADS <= 63 && STAGES >= 2 && STAGES <= 4, "vmcnt counts to 63");
 };
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES>
@@ -312,12 +312,10 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
         constexpr bool MORE = decltype(more)::value;
         const int here = stage;
         if (++stage == STAGES) stage = 0;
-        // scale bytes behind the last block belong to nothing: 2^-127 for their zero codes
-        const int blocks = LEFT > 0 ? 2 : p.last_blocks - 2 * g, held = blocks >= 2 ? 0xffff : blocks == 1 ? 0xff : 0;
 #pragma unroll
-        for (int i = 0; i < FM; ++i) sx[i] = LEFT > 0 ? sx_next[i] : sx_next[i] & held;
+        for (int i = 0; i < FM; ++i) sx[i] = sx_next[i];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sw[j] = LEFT > 0 ? sw_next[j] : sw_next[j] & held;
+        for (int j = 0; j < FN; ++j) sw[j] = sw_next[j];
         read_w(here, 1);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -347,6 +345,8 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     };
     int left = p.nkt - 1;
     for (; left >= STAGES; --left) k_tile(std::integral_constant<int, STAGES - 1>(), std::true_type());
+    if constexpr (STAGES > 3)
+        if (left >= 3) { k_tile(std::integral_constant<int, 3>(), std::false_type()); --left; }
     if constexpr (STAGES > 2)
         if (left >= 2) { k_tile(std::integral_constant<int, 2>(), std::false_type()); --left; }
     if (left >= 1) k_tile(std::integral_constant<int, 1>(), std::false_type());
@@ -451,7 +451,6 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
     p.ldx = d->ldx; p.ld_xs = d->ld_xs; p.ldw = d->ldw; p.ld_ws = d->ld_ws;
     p.m = d->m; p.n_out = d->epi == DM_EPI_GEGLU ? d->n / 2 : d->n; p.n_pad = p.n_out;
     p.nkt = kp / MX_PAD;
-    p.last_blocks = (d->k + MX_BLOCK - 1) / MX_BLOCK - (p.nkt - 1) * (MX_PAD / MX_BLOCK);
     p.bias = d->bias; p.r = d->r; p.ldr = d->ldr; p.c = d->c; p.ldc = d->ldc; p.cs = d->c_scales; p.ld_cs = d->ld_cs;
     p.epi = d->epi; p.c_type = d->c_type;
     if (fmt_ok(d->c_type)) {
