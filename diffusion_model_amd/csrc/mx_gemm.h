@@ -16,6 +16,7 @@ struct MxArgs {
     long ldx, ld_xs, ldw, ld_ws;
     int m, n_out, n_pad;  // rows of C; columns of C; columns to write (MX results: padded, the padding as zeros)
     int nkt;              // k-tiles of 128 values
+    int last_blocks;      // blocks of 32 in the last of them that hold values: 1 to 4
     int tiles_m, tiles_n;
     const float* bias;
     const void* r;

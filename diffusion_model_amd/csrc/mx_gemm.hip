@@ -312,10 +312,12 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
         constexpr bool MORE = decltype(more)::value;
         const int here = stage;
         if (++stage == STAGES) stage = 0;
+        // scale bytes behind the last block belong to nothing: 2^-127 for their zero codes
+        const int blocks = LEFT > 0 ? 2 : p.last_blocks - 2 * g, held = blocks >= 2 ? 0xffff : blocks == 1 ? 0xff : 0;
 #pragma unroll
-        for (int i = 0; i < FM; ++i) sx[i] = sx_next[i];
+        for (int i = 0; i < FM; ++i) sx[i] = LEFT > 0 ? sx_next[i] : sx_next[i] & held;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sw[j] = sw_next[j];
+        for (int j = 0; j < FN; ++j) sw[j] = LEFT > 0 ? sw_next[j] : sw_next[j] & held;
         read_w(here, 1);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -451,6 +453,7 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
     p.ldx = d->ldx; p.ld_xs = d->ld_xs; p.ldw = d->ldw; p.ld_ws = d->ld_ws;
     p.m = d->m; p.n_out = d->epi == DM_EPI_GEGLU ? d->n / 2 : d->n; p.n_pad = p.n_out;
     p.nkt = kp / MX_PAD;
+    p.last_blocks = (d->k + MX_BLOCK - 1) / MX_BLOCK - (p.nkt - 1) * (MX_PAD / MX_BLOCK);
     p.bias = d->bias; p.r = d->r; p.ldr = d->ldr; p.c = d->c; p.ldc = d->ldc; p.cs = d->c_scales; p.ld_cs = d->ld_cs;
     p.epi = d->epi; p.c_type = d->c_type;
     if (fmt_ok(d->c_type)) {

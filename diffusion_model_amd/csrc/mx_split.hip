@@ -211,15 +211,17 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
         typename MxFragment<XF>::type x[FM];
         typename MxFragment<WF>::type w[FN];
         int sx[FM], sw[FN];
+        // a lane's scale bytes are those of block g; behind the last block they belong to nothing: 2^-127 for its zero codes
+        const int held = wave + SPLIT_WAVES * s < p.nkt - 1 || g < p.last_blocks ? 0xff : 0;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             x[i] = lds_fragment16<XF, EXACT>(at + i * 16 * G::XB, fr, g);
-            sx[i] = group[i * 256 + fr * 16 + (s & 3) * 4 + g];
+            sx[i] = group[i * 256 + fr * 16 + (s & 3) * 4 + g] & held;
         }
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
             w[j] = lds_fragment16<WF, EXACT>(at + FM * 16 * G::XB + j * 16 * G::WB, fr, g);
-            sw[j] = group[(FM + j) * 256 + fr * 16 + (s & 3) * 4 + g];
+            sw[j] = group[(FM + j) * 256 + fr * 16 + (s & 3) * 4 + g] & held;
         }
         if (s + G::DEPTH < count) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments are in registers: the slot may be refilled

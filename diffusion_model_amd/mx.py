@@ -39,8 +39,8 @@ class MXTensor:
     """A quantised matrix of ``rows`` rows of ``k`` values.
 
     ``codes``: uint8 ``[rows, kp]`` (mxfp8) or ``[rows, kp / 2]`` (mxfp4; the even value in the low nibble) with kp = k rounded
-    up to 128 and zeros behind column k; ``scales``: uint8 ``[rows, kp / 32]``.  Both may have a row stride (a multiple of 16 and
-    of 4 bytes).  Matrices quantised elsewhere in this format are wrapped as they are."""
+    up to 128 and zeros behind column k; ``scales``: uint8 ``[rows, kp / 32]``, anything behind the last block that holds values.  Both
+    may have a row stride (a multiple of 16 and of 4 bytes).  Matrices quantised elsewhere in this format are wrapped as they are."""
     # Results of this module hold one buffer, codes then scales, and make the two views when somebody asks for them: an
     # allocation or a view costs a small call more than a microsecond each.
     __slots__ = ("_buffer", "_codes", "_scales", "rows", "k", "fmt", "device")

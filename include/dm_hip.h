@@ -298,7 +298,8 @@ int dm_layernorm(const void* x, long ldx, void* y, long ldy, int rows, int c, in
  * clip.py:76-88) run on 4- or 8-bit values.  No counterpart in the reference, which computes in fp32.
  * A matrix of `rows` rows of k values is held as `codes` (rows of ldc bytes) and `scales` (rows of lds bytes).  Rows are padded
  * to kp = k rounded up to 128: kp bytes (DM_MXFP8) or kp/2 bytes (DM_MXFP4) of codes and kp/32 scale bytes.  The padding of
- * the codes must be zero; every entry point here that writes such a matrix writes its padding.  codes 16-byte aligned, ldc a
+ * the codes must be zero, scale bytes behind the last block may be anything; every entry point here that writes such a matrix
+ * writes zeros there.  codes 16-byte aligned, ldc a
  * multiple of 16; scales 4-byte aligned, lds a multiple of 4.
  * Quantisation of a block of 32 values: byte = max(0, biased exponent of the largest magnitude - 8 (MXFP8) or 2 (MXFP4)); a
  * value v becomes v * 2^(127 - byte) rounded to the nearest code, ties to even, saturated at the largest; a block that holds
