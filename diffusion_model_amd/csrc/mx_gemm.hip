@@ -148,7 +148,7 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     static_assert(BM % 64 == 0 && BN % 64 == 0 && WM % 32 == 0 && WN % 32 == 0, "whole requests and fragments");
     static_assert(PX * WAVES * 1024 == BM * XB && PW * WAVES * 1024 == BN * WB && (BM + BN) / 64 <= WAVES, "every wave requests the same");
     static_assert(WN % 64 == 0, "a wave holds both the values and the gates of its columns");
-    static_assert((STAGES - 1) * LOADS <= 63 && STAGES >= 2 && STAGES <= 4, "vmcnt counts to 63");
+    static_assert((STAGES - 1) * LOADS <= 63 && (STAGES == 2 || STAGES == 3), "vmcnt counts to 63; the tail of the k loop");
 };
 
 template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES>
@@ -347,8 +347,6 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     };
     int left = p.nkt - 1;
     for (; left >= STAGES; --left) k_tile(std::integral_constant<int, STAGES - 1>(), std::true_type());
-    if constexpr (STAGES > 3)
-        if (left >= 3) { k_tile(std::integral_constant<int, 3>(), std::false_type()); --left; }
     if constexpr (STAGES > 2)
         if (left >= 2) { k_tile(std::integral_constant<int, 2>(), std::false_type()); --left; }
     if (left >= 1) k_tile(std::integral_constant<int, 1>(), std::false_type());
