@@ -7,7 +7,8 @@ namespace {
 
 constexpr int THREADS = 256;
 
-// Eight consecutive values at p, of which those below `left` exist (the others read as zero).
+// Eight consecutive values at p, of which those below `left` exist (the others read as zero).  The conversion from bf16 stands
+// in the branch on `left`, so a bf16 load is waited for before the next one is issued; fp32 loads of several groups are in flight together.
 template <typename T> __device__ __forceinline__ void load8(const T* p, int left, float* v) {
     constexpr int EPC = ElemTraits<T>::EPC;
     if (left >= 8) {
@@ -32,9 +33,10 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int left, con
 
 // ---- quantise / dequantise ------------------------------------------------------------------------------------------
 // A lane holds eight values, a quad the 32 of a block.  `gpr` = groups of eight per padded row (a multiple of 16), so a
-// quad never straddles rows; a block sweeps UNROLL x 256 consecutive groups with all its loads ahead of the arithmetic.
-// Bound by HBM: 65536 x 1280 bf16 to 4 bits 50 us (212 MB, 4.2 TB/s; a large copy reaches 5.1 here), back 32 us (6.6 TB/s, what was
-// just written is still cached); 1003 x 1283 fp32 3.3 us, of which 2.5 are the launch.
+// quad never straddles rows; a block sweeps UNROLL x 256 consecutive groups with all its loads ahead of the arithmetic (fp32 and
+// dequantisation; bf16 rows: one 16-byte load at a time per lane, see load8).  Bound by HBM: 65536 x 1280 bf16 to 4 bits 50 us
+// (212 MB, 4.2 TB/s; a large copy reaches 5.1 here), back 32 us (6.6 TB/s, what was just written is still cached); 1003 x 1283 fp32
+// 3.2 us, of which 2.5 are the launch.
 struct Groups {
     int gpr;
     uint32_t magic;  // ceil(2^32 / gpr)
@@ -253,8 +255,9 @@ __device__ __forceinline__ void norm_store(const NormArgs& p, long row, int at, 
 
 // The row stays in registers: TPR threads of NV groups of eight values, so x and the residual are read once, and the layer
 // norm's variance is a second sum over registers, not a difference of moments.  Bound by HBM: 16384 x 8192 bf16 with residual to
-// e4m3 190 us (944 MB, 5.0 TB/s; a large copy reaches 5.1); short ones by the chain load - sum - store: 1 x 1280 2.8 us, 1024 x
-// 1280 fp32 6 us (21 MB).  A wave per row up to 1024 values needs no barrier; longer rows are spread over four, so that no
+// e4m3 180 to 199 us (944 MB, 4.7 to 5.2 TB/s; a large copy reaches 5.1), LayerNorm 205 to 208; short ones by the chain load - sum - store:
+// 1 x 1280 2.8 us, 1024 x 1280 fp32 6.1 us (21 MB).  Sums in 64 bits cost 65536 x 1280 LayerNorm to e2m1 7 to 9 % (164 us in
+// 32), the others at most 3 %.  A wave per row up to 1024 values needs no barrier; longer rows are spread over four, so that no
 // lane has more than 64.
 template <typename T, int OUT, int TPR, int NV>
 __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(THREADS) void row_norm_kernel(NormArgs p) {
 
 // Rows too long for registers: one block per row sweeps it once per sum and once for the output; the sweeps behind the
 // first are served by the caches.  With a residual they read the stored h (each thread what it wrote itself), so h may be x
-// or the residual itself here as in the kernel above.
+// or the residual itself here as in the kernel above.  1024 x 32768 bf16 with residual: RMS norm 60 us, LayerNorm 72 (268 MB, 4.5 and 3.7 TB/s).
 template <typename T, int OUT> __global__ __launch_bounds__(THREADS) void row_norm_loop_kernel(NormArgs p) {
     __shared__ double red[THREADS / 64];
     const long row = p.first + blockIdx.x;

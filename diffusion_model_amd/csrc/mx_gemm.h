@@ -108,7 +108,8 @@ __device__ __forceinline__ float gelu_f32(float x) {
 // GELU(erf) = x Phi(x) for results of 16 bits and fewer: Phi(-t) = 2^P(t), P of degree 9, fitted on 0 <= t <= 13 to log2 of it.  Evaluated
 // in fp32 it is within 6e-6 of the result up to t = 3 and 6e-5 up to 13, a 60th of bf16's rounding; behind 13, where
 // Phi leaves the normal range, P falls on to -infinity.  (A polynomial for Phi itself, three instructions and the exponential less, is
-// within 1.4e-5 |x|, which is 0.4 % of the result at -3 and 30 % at -4.)
+// within 1.4e-5 |x|, which is 0.4 % of the result at -3 and 30 % at -4.  It is 4 % faster at 65536 x 2560 x 320 with GEGLU for e4m3 x e2m1,
+// 11 % for 4-bit and 15 % for 8-bit pairs.)
 __device__ __forceinline__ float gelu_exp2_f(float x) {
     const float t = fabsf(x);
     float p = -2.1005828187981024e-09f;

@@ -376,14 +376,16 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     return dm_check_launch();
 }
 // Which tile, by measurement on a warm card (e4m3 x e2m1 and a bf16 result where nothing else is said):
-//   256 x 256  one block per CU.  Where its rounds over the 256 CUs are full and k is long: 8192^3 in 289 us against 358 for
-//              the next (4 bits), 400 against 437 (e4m3 x e2m1); 16384 x 5120 x 5120: 351 against 360
+//   256 x 256  one block per CU.  Where its rounds over the 256 CUs are full and k is long: 8192^3 in 279 us against 342 for
+//              the next (4 bits), 386 against 424 (e4m3 x e2m1); 16384 x 5120 x 5120: 313 against 342
 //   128 x 256  two blocks per CU, so that one's epilogue runs beside the other's k loop; W in 4 bits only, whose four
-//              fragments per wave fit the 128 registers that leaves (16384 x 5120 x 320: 54 us against 57 for 256 x 256 and 56 for
-//              128 x 128; 65536 x 2560 x 320 with GEGLU: 94, 96, 106; 65536 x 2560 x 1280 to bf16: 241, 240)
-//   128 x 128  two blocks per CU, once there is one for each (4096 x 1280 x 1280: 12.2 us against 12.9 for 64 x 64; x 5120: 33
-//              against 41)
-//   64 x 64    the rest (1024 x 1280 x 1280: 7.2 us against 7.5; x 5120: 18.6 against 28.2)
+//              fragments per wave fit the 128 registers that leaves (16384 x 5120 x 320: 50 us against 54 for 256 x 256 and 54 for
+//              128 x 128; 65536 x 2560 x 320 with GEGLU: 93, 103, 101; at k = 1280 it is level with 256 x 256: 65536 x 2560 233 and 232,
+//              16384 x 5120 108 and 105)
+//   128 x 128  two blocks per CU, once there is one for each (4096 x 1280 x 1280: 12.2 us against 12.4 for 64 x 64; x 5120: 32.4
+//              against 38.8)
+//   64 x 64    the rest (1024 x 1280 x 1280: 7.2 us against 7.6; x 5120: 18.8 against 28.3; a short k is the exception, 512 x 1280 x 320
+//              4.9 to 6.0 against 4.8)
 template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_t s) {
     const int wide = p.epi == DM_EPI_GEGLU ? 2 * p.n_pad : p.n_pad;
     auto tiles = [&](int bm, int bn) { return (long)((p.m + bm - 1) / bm) * ((wide + bn - 1) / bn); };
@@ -403,9 +405,9 @@ template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream
     return launch_fmt<XF, WF, false>(p, s);
 }
 // The split kernel's tile: the smallest that needs at most one block per CU, since blocks read their operands anew
-// (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.4 in 200, the 64 x 64 tile 14.4; 128 x 8192 x 8192 with the largest 17.5 against 31.5;
-// 256 x 8192 x 8192 in 512 of those 32.5 against 32.3, 1024 x 1280 x 5120 in 320 of them 23 against 18.6).  The largest is slower than
-// the 64 x 64 tile on a short k (512 x 1280 x 1280: 6.1 us against 5.8; x 5120: 9.8 against 14.6).  Up to 16 rows a tile of 16 x 64 is
+// (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.4 in 200, the 64 x 64 tile 14.4; 128 x 8192 x 8192 with the largest 17.3 against 31.2;
+// 256 x 8192 x 8192 in 512 of those 32.2 against 32.2, 1024 x 1280 x 5120 in 320 of them 23 against 18.8).  The largest is slower than
+// the 64 x 64 tile on a short k (512 x 1280 x 1280: 6.0 us against 5.8; x 5120: 9.8 against 14.6).  Up to 16 rows a tile of 16 x 64 is
 // taken at any size: W is read once then, and that is all there is to do.
 bool split_tile(const MxArgs& p, int* fm, int* fn) {
     static const int shapes[][2] = {{1, 1}, {1, 2}, {2, 2}, {1, 4}, {2, 4}, {4, 4}};

@@ -10,8 +10,9 @@ A matrix is quantised in blocks of 32 consecutive values of a row that share a p
 e = floor(log2(largest magnitude)) - 8 (mxfp8) or - 2 (mxfp4), at least -127, stored as the byte e + 127; values are rounded to
 nearest even and saturated.  A block that holds an infinity or a NaN stands for NaN (byte 255).
 
-Matrices are 2-D row-major views ``[rows, k]`` with any row stride, as everywhere in this package; tensors live on the HIP
-device, results are new tensors, launches go to the current stream of the operands' device.  Nothing here has a backward pass.
+Matrices are 2-D row-major views ``[rows, k]`` with any row stride, as everywhere in this package; norm weights and biases are float32
+whatever the rows' type; tensors live on the HIP device, results are new tensors, launches go to the current stream of the
+operands' device.  Nothing here has a backward pass.
 """
 from __future__ import annotations
 
@@ -238,7 +239,9 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
     ``activation``: None, ``"quick_gelu"`` (v sigmoid(1.702 v)) or ``"geglu"`` (the first n / 2 columns times gelu(the others):
     ``[m, n / 2]``).  The result has ``out_dtype`` (bfloat16 / float32; ``residual`` has the same type), or is an
     :class:`MXTensor` with ``out_format`` (no residual).  Accumulation is fp32; bf16 and MX results come from the scaled matrix
-    instructions, which lose about 2e-5 of an 8-bit product, fp32 results are exact to fp32."""
+    instructions, which lose about 2e-5 of an 8-bit product.  fp32 results are fp32 sums of exact products, with activations right to a few
+    units; for them an 8-bit operand's values are held in bf16, so those of scale bytes 0 to 2 are rounded to multiples of 2^-133 and those
+    past bf16's largest (byte 247 on, which ``quantize`` never writes) are infinite."""
     what = "mx.linear"
     if activation not in _ACTIVATIONS:
         raise ValueError(f"{what}: unknown activation {activation!r}")

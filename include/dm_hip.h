@@ -299,12 +299,11 @@ int dm_layernorm(const void* x, long ldx, void* y, long ldy, int rows, int c, in
  * A matrix of `rows` rows of k values is held as `codes` (rows of ldc bytes) and `scales` (rows of lds bytes).  Rows are padded
  * to kp = k rounded up to 128: kp bytes (DM_MXFP8) or kp/2 bytes (DM_MXFP4) of codes and kp/32 scale bytes.  The padding of
  * the codes must be zero, scale bytes behind the last block may be anything; every entry point here that writes such a matrix
- * writes zeros there.  codes 16-byte aligned, ldc a
- * multiple of 16; scales 4-byte aligned, lds a multiple of 4.
+ * writes zeros there.  codes 16-byte aligned, ldc a multiple of 16; scales 4-byte aligned, lds a multiple of 4.
  * Quantisation of a block of 32 values: byte = max(0, biased exponent of the largest magnitude - 8 (MXFP8) or 2 (MXFP4)); a
  * value v becomes v * 2^(127 - byte) rounded to the nearest code, ties to even, saturated at the largest; a block that holds
  * an infinity or a NaN gets byte 255 and zero codes and stands for NaN.
- * x: rows of ldx fp32 / bf16 elements, any alignment (16-byte aligned rows with k a multiple of 8 are read 16 bytes at a time). */
+ * x: rows of ldx fp32 / bf16 elements, any alignment. */
 int dm_mx_quantize(const void* x, long ldx, long rows, int k, int dtype, int fmt, unsigned char* codes, long ldc,
                    unsigned char* scales, long lds, hipStream_t stream);
 /* The values that the codes stand for, as fp32 or bf16 (exact in both wherever the value is not a subnormal of the type). */
@@ -342,8 +341,11 @@ int dm_row_norm(const DmRowNormDesc* d, hipStream_t stream);
  * n/2 columns).  bias: n fp32 or NULL.  c_type: DM_BF16 / DM_F32 (rows of ldc elements; r, optional, has the same type), or
  * DM_MXFP8 / DM_MXFP4 (c = codes, ldc bytes; c_scales, ld_cs; no r): an MX matrix ready to be the next product's X.
  * Accumulation in fp32.  DM_BF16 and MX results come from the scaled matrix instructions on the codes themselves, whose adder
- * drops low bits of e4m3 products (2e-5 of the result on normal data); DM_F32 results with an e4m3 operand from bf16 matrix instructions on
- * the decoded operands, which are exact there. */
+ * drops low bits of e4m3 products (2e-5 of the result on normal data); their GELU is within 6e-5 of its result.  DM_F32 results with an
+ * e4m3 operand come from bf16 matrix instructions on the decoded operands: products exact, sums in fp32; activations within a few
+ * units.  bf16 holds every decoded value but at the ends of the scales' range: in DM_F32 results e4m3 values of scale bytes 0 to 2
+ * are rounded to multiples of 2^-133, and values past bf16's largest are infinite (e4m3 from byte 247 on, e2m1 at 254, which no
+ * entry point here writes). */
 #define DM_X_MX 0
 #define DM_X_BF16 1
 #define DM_X_F32 2
