@@ -112,16 +112,10 @@ __device__ __forceinline__ void store_fragments(const MxArgs& p, const f32x16 (&
             store16<CT>(p, row(i), column(j), v, lane, edge);
         }
 }
-// RESULTS: the types that the kernel is launched for (fp32 results of e4m3 operands have kernels of their own)
-template <int EPI, MxResults RESULTS, int FM, int FN, typename Row, typename Column>
+template <int EPI, bool F32, int FM, int FN, typename Row, typename Column>
 __device__ __forceinline__ void store_typed(const MxArgs& p, const f32x16 (&acc)[FM][FN], Row row, Column column, int lane, bool edge) {
-    if constexpr (RESULTS == MxResults::FP32) {
-        store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
-        return;
-    }
-    if constexpr (RESULTS == MxResults::ANY)
-        if (p.c_type == DM_F32) return store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
-    if (p.c_type == DM_BF16) store_fragments<EPI, DM_BF16>(p, acc, row, column, lane, edge);
+    if constexpr (F32) store_fragments<EPI, DM_F32>(p, acc, row, column, lane, edge);
+    else if (p.c_type == DM_BF16) store_fragments<EPI, DM_BF16>(p, acc, row, column, lane, edge);
     else if (p.c_type == DM_MXFP8) store_fragments<EPI, DM_MXFP8>(p, acc, row, column, lane, edge);
     else store_fragments<EPI, DM_MXFP4>(p, acc, row, column, lane, edge);
 }
@@ -134,7 +128,7 @@ __device__ __forceinline__ void store_typed(const MxArgs& p, const f32x16 (&acc)
 // at 8192^3, 4 bits: a fifth of the kernel's time).  They are fetched for a group of four k-tiles, 16 bytes of a row, a
 // quarter of the tile's rows with every k-tile: "quarter" q = 4 group + c is requested with k-tile q - 3 and is used with k-tile 4
 // group at the earliest, when every request up to that k-tile's has landed.
-template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> struct MxTile {
+template <int XF, int WF, bool F32, int BM, int BN, int WM, int WN, int STAGES> struct MxTile {
     static constexpr int XB = mx_bytes(XF, MX_PAD), WB = mx_bytes(WF, MX_PAD);
     static constexpr int WAVES = (BM / WM) * (BN / WN);
     static constexpr int STAGE = BM * XB + BN * WB;  // bytes
@@ -151,9 +145,10 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
     static_assert((STAGES - 1) * LOADS <= 63 && (STAGES == 2 || STAGES == 3), "vmcnt counts to 63; the tail of the k loop");
 };
 
-template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::WAVES), (MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::WAVES * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>::BLOCKS + 3) / 4) void mx_gemm_kernel(MxArgs p) {
-    typedef MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES> G;
+template <int XF, int WF, bool F32, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__((64 * MxTile<XF, WF, F32, BM, BN, WM, WN, STAGES>::WAVES), (MxTile<XF, WF, F32, BM, BN, WM, WN, STAGES>::WAVES * MxTile<XF, WF, F32, BM, BN, WM, WN, STAGES>::BLOCKS + 3) / 4) void mx_gemm_kernel(MxArgs p) {
+    typedef MxTile<XF, WF, F32, BM, BN, WM, WN, STAGES> G;
+    constexpr bool EXACT = mx_exact(XF, WF, F32);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 5, fr = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -353,26 +348,25 @@ __global__ __launch_bounds__((64 * MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES>
     k_tile(std::integral_constant<int, 0>(), std::false_type());
 
     // ---- epilogue: a lane holds row .. + fr and 16 columns per fragment
-    constexpr MxResults RESULTS = mx_results(XF, WF, EXACT);
     const bool edge = col0 + (geglu ? BN / 2 : BN) > p.n_out;
     auto row = [&](int i) { return (long)(m0 + wm * WM + i * 32 + fr); };
-    if (geglu) store_typed<DM_EPI_GEGLU, RESULTS>(p, acc, row, column, lane, edge);
-    else if (p.epi == DM_EPI_QUICKGELU) store_typed<DM_EPI_QUICKGELU, RESULTS>(p, acc, row, column, lane, edge);
-    else store_typed<DM_EPI_PLAIN, RESULTS>(p, acc, row, column, lane, edge);
+    if (geglu) store_typed<DM_EPI_GEGLU, F32>(p, acc, row, column, lane, edge);
+    else if (p.epi == DM_EPI_QUICKGELU) store_typed<DM_EPI_QUICKGELU, F32>(p, acc, row, column, lane, edge);
+    else store_typed<DM_EPI_PLAIN, F32>(p, acc, row, column, lane, edge);
 }
 
-template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {
-    typedef MxTile<XF, WF, EXACT, BM, BN, WM, WN, STAGES> G;
+template <int XF, int WF, bool F32, int BM, int BN, int WM, int WN, int STAGES> int launch(MxArgs p, hipStream_t s) {
+    typedef MxTile<XF, WF, F32, BM, BN, WM, WN, STAGES> G;
     constexpr int LDS = G::LDS;
     const int bo = p.epi == DM_EPI_GEGLU ? BN / 2 : BN;
     p.tiles_m = (p.m + BM - 1) / BM;
     p.tiles_n = (p.n_pad + bo - 1) / bo;
     if (!mx_grid_ok((long)p.tiles_m * p.tiles_n, 64 * G::WAVES)) return DM_ERR_ARG;
     static DmLdsAttr attr;
-    const void* fn = reinterpret_cast<const void*>(&mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES>);
+    const void* fn = reinterpret_cast<const void*>(&mx_gemm_kernel<XF, WF, F32, BM, BN, WM, WN, STAGES>);
     if (LDS > 64 * 1024)
         if (const int rc = dm_set_lds_attr(fn, attr, LDS)) return rc;
-    mx_gemm_kernel<XF, WF, EXACT, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
+    mx_gemm_kernel<XF, WF, F32, BM, BN, WM, WN, STAGES><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * G::WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }
 // Which tile, by measurement on a warm card (e4m3 x e2m1 and a bf16 result where nothing else is said):
@@ -386,23 +380,21 @@ template <int XF, int WF, bool EXACT, int BM, int BN, int WM, int WN, int STAGES
 //              against 38.8)
 //   64 x 64    the rest (1024 x 1280 x 1280: 7.2 us against 7.6; x 5120: 18.8 against 28.3; a short k is the exception, 512 x 1280 x 320
 //              4.9 to 6.0 against 4.8)
-template <int XF, int WF, bool EXACT> int launch_fmt(const MxArgs& p, hipStream_t s) {
+template <int XF, int WF, bool F32> int launch_fmt(const MxArgs& p, hipStream_t s) {
     const int wide = p.epi == DM_EPI_GEGLU ? 2 * p.n_pad : p.n_pad;
     auto tiles = [&](int bm, int bn) { return (long)((p.m + bm - 1) / bm) * ((wide + bn - 1) / bn); };
-    if constexpr (!EXACT) {
+    if constexpr (!mx_exact(XF, WF, F32)) {
         const long t256 = tiles(256, 256), rounds = (t256 + 255) / 256;
         if (t256 * 5 >= rounds * 256 * 4 && (WF == 8 || p.nkt >= 32))
-            return launch<XF, WF, EXACT, 256, 256, 128, 64, XF == 4 && WF == 4 ? 3 : 2>(p, s);
+            return launch<XF, WF, F32, 256, 256, 128, 64, XF == 4 && WF == 4 ? 3 : 2>(p, s);
         if constexpr (WF == 4)
-            if (tiles(128, 256) >= 512) return launch<XF, WF, EXACT, 128, 256, 32, 128, 2>(p, s);
+            if (tiles(128, 256) >= 512) return launch<XF, WF, F32, 128, 256, 32, 128, 2>(p, s);
     }
-    if (tiles(128, 128) >= 256) return launch<XF, WF, EXACT, 128, 128, 64, 64, 2>(p, s);
-    return launch<XF, WF, EXACT, 64, 64, 32, 64, 2>(p, s);
+    if (tiles(128, 128) >= 256) return launch<XF, WF, F32, 128, 128, 64, 64, 2>(p, s);
+    return launch<XF, WF, F32, 64, 64, 32, 64, 2>(p, s);
 }
-template <int XF, int WF> int launch_tile(const MxArgs& p, bool exact, hipStream_t s) {
-    if constexpr (XF == 8 || WF == 8)
-        if (exact) return launch_fmt<XF, WF, true>(p, s);
-    return launch_fmt<XF, WF, false>(p, s);
+template <int XF, int WF> int launch_tile(const MxArgs& p, bool f32, hipStream_t s) {
+    return f32 ? launch_fmt<XF, WF, true>(p, s) : launch_fmt<XF, WF, false>(p, s);
 }
 // The split kernel's tile: the smallest that needs at most one block per CU, since blocks read their operands anew
 // (77 x 1280 x 5120: 7.7 us in 400 blocks, 5.4 in 200, the 64 x 64 tile 14.4; 128 x 8192 x 8192 with the largest 17.3 against 31.2;
@@ -467,9 +459,9 @@ extern "C" int dm_mx_gemm(const DmMxGemmDesc* d, hipStream_t stream) {
         p.ldx = d->ldx * (d->x_src == DM_X_F32 ? 4 : 2);  // bytes, as for codes
         p.k = d->k;
     }
-    const bool exact = d->c_type == DM_F32;
+    const bool f32 = d->c_type == DM_F32;
     int fm, fn;
-    if (split_tile(p, &fm, &fn)) return dm_mx_split_launch(p, d->x_fmt, d->w_fmt, exact, d->x_src, fm, fn, stream);
-    if (d->x_fmt == DM_MXFP8) return d->w_fmt == DM_MXFP8 ? launch_tile<8, 8>(p, exact, stream) : launch_tile<8, 4>(p, exact, stream);
-    return d->w_fmt == DM_MXFP8 ? launch_tile<4, 8>(p, exact, stream) : launch_tile<4, 4>(p, exact, stream);
+    if (split_tile(p, &fm, &fn)) return dm_mx_split_launch(p, d->x_fmt, d->w_fmt, f32, d->x_src, fm, fn, stream);
+    if (d->x_fmt == DM_MXFP8) return d->w_fmt == DM_MXFP8 ? launch_tile<8, 8>(p, f32, stream) : launch_tile<8, 4>(p, f32, stream);
+    return d->w_fmt == DM_MXFP8 ? launch_tile<4, 8>(p, f32, stream) : launch_tile<4, 4>(p, f32, stream);
 }

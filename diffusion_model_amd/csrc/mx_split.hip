@@ -70,8 +70,8 @@ __device__ __forceinline__ void mma16(f32x4& acc, const typename MxFragment<XF>:
     }
 }
 // Columns col .. col + 7 of row m; the four lanes of a quad hold the 32 columns of an MX block.
-__device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* v, int lane, bool f32) {
-    if (!f32 && (p.c_type == DM_MXFP8 || p.c_type == DM_MXFP4)) {
+template <bool F32> __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* v, int lane) {
+    if (!F32 && p.c_type != DM_BF16) {
         if (col >= p.n_pad) return;  // whole quads
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = col + e < p.n_out ? v[e] : 0.f;
@@ -81,7 +81,7 @@ __device__ __forceinline__ void store8(const MxArgs& p, long m, int col, float* 
         return;
     }
     const int left = p.n_out - col;
-    if (!f32) {
+    if (!F32) {
         bf16_t* dst = static_cast<bf16_t*>(p.c) + m * p.ldc + col;
         float r[8] = {};
         if (p.r) load_values<bf16_t, 8>(static_cast<const bf16_t*>(p.r) + m * p.ldr + col, left, r);
@@ -122,9 +122,10 @@ template <int XF, int WF, int FM, int FN> struct SplitRing {
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
-template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN>
+template <int XF, int WF, bool F32, int XSRC, int FM, int FN>
 __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
     typedef SplitRing<XF, WF, FM, FN> G;
+    constexpr bool EXACT = mx_exact(XF, WF, F32);
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, g = lane >> 4, fr = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -261,23 +262,21 @@ __global__ __launch_bounds__(64 * SPLIT_WAVES) void mx_split_kernel(MxArgs p) {
                 for (int e = 0; e < 4; ++e) v[4 * h + e] += t[e];
             }
     };
-    constexpr MxResults RESULTS = mx_results(XF, WF, EXACT);
-    const bool f32 = RESULTS == MxResults::FP32 || (RESULTS == MxResults::ANY && p.c_type == DM_F32);
     float v[8];
     total(geglu ? 2 * (c8 >> 1) : c8 >> 1, col, v);
     if (geglu) {
         float gate[8];
         total(2 * (c8 >> 1) + 1, p.n_out + col, gate);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f32 ? gelu_f32(gate[e]) : gelu_exp2_f(gate[e]);
+        for (int e = 0; e < 8; ++e) v[e] *= F32 ? gelu_f32(gate[e]) : gelu_exp2_f(gate[e]);
     } else if (p.epi == DM_EPI_QUICKGELU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = f32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));
+        for (int e = 0; e < 8; ++e) v[e] = F32 ? quick_gelu_f32(v[e]) : v[e] / (1.f + __expf(-1.702f * v[e]));
     }
-    store8(p, m0 + row, col, v, threadIdx.x, f32);
+    store8<F32>(p, m0 + row, col, v, threadIdx.x);
 }
 
-template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN> int launch_split(MxArgs p, hipStream_t s) {
+template <int XF, int WF, bool F32, int XSRC, int FM, int FN> int launch_split(MxArgs p, hipStream_t s) {
     constexpr int LDS = SplitRing<XF, WF, FM, FN>::LDS;
     static_assert(32 * FM * FN <= 64 * SPLIT_WAVES, "one thread per eight columns");
     const int bo = p.epi == DM_EPI_GEGLU ? FN * 8 : FN * 16;
@@ -286,39 +285,37 @@ template <int XF, int WF, bool EXACT, int XSRC, int FM, int FN> int launch_split
     if (!mx_grid_ok((long)p.tiles_m * p.tiles_n, 64 * SPLIT_WAVES)) return DM_ERR_ARG;
     static DmLdsAttr attr;
     if (LDS > 64 * 1024)
-        if (const int rc = dm_set_lds_attr(reinterpret_cast<const void*>(&mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN>), attr, LDS)) return rc;
-    mx_split_kernel<XF, WF, EXACT, XSRC, FM, FN><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * SPLIT_WAVES, LDS, s>>>(p);
+        if (const int rc = dm_set_lds_attr(reinterpret_cast<const void*>(&mx_split_kernel<XF, WF, F32, XSRC, FM, FN>), attr, LDS)) return rc;
+    mx_split_kernel<XF, WF, F32, XSRC, FM, FN><<<dim3((unsigned)(p.tiles_m * p.tiles_n)), 64 * SPLIT_WAVES, LDS, s>>>(p);
     return dm_check_launch();
 }
 
-template <int XF, int WF, bool EXACT, int XSRC> int launch_tile(const MxArgs& p, int fm, int fn, hipStream_t s) {
+template <int XF, int WF, bool F32, int XSRC> int launch_tile(const MxArgs& p, int fm, int fn, hipStream_t s) {
     if (fm == 1) {
-        if (fn == 1) return launch_split<XF, WF, EXACT, XSRC, 1, 1>(p, s);
-        if (fn == 2) return launch_split<XF, WF, EXACT, XSRC, 1, 2>(p, s);
-        if (fn == 4) return launch_split<XF, WF, EXACT, XSRC, 1, 4>(p, s);
+        if (fn == 1) return launch_split<XF, WF, F32, XSRC, 1, 1>(p, s);
+        if (fn == 2) return launch_split<XF, WF, F32, XSRC, 1, 2>(p, s);
+        if (fn == 4) return launch_split<XF, WF, F32, XSRC, 1, 4>(p, s);
     }
     if constexpr (XSRC == DM_X_MX) {
-        if (fm == 2 && fn == 2) return launch_split<XF, WF, EXACT, XSRC, 2, 2>(p, s);
-        if (fm == 2 && fn == 4) return launch_split<XF, WF, EXACT, XSRC, 2, 4>(p, s);
-        if (fm == 4 && fn == 4) return launch_split<XF, WF, EXACT, XSRC, 4, 4>(p, s);
+        if (fm == 2 && fn == 2) return launch_split<XF, WF, F32, XSRC, 2, 2>(p, s);
+        if (fm == 2 && fn == 4) return launch_split<XF, WF, F32, XSRC, 2, 4>(p, s);
+        if (fm == 4 && fn == 4) return launch_split<XF, WF, F32, XSRC, 4, 4>(p, s);
     }
     return DM_ERR_ARG;
 }
-template <int XF, int WF, bool EXACT> int launch_src(const MxArgs& p, int x_src, int fm, int fn, hipStream_t s) {
-    if (x_src == DM_X_BF16) return launch_tile<XF, WF, EXACT, DM_X_BF16>(p, fm, fn, s);
-    if (x_src == DM_X_F32) return launch_tile<XF, WF, EXACT, DM_X_F32>(p, fm, fn, s);
-    return launch_tile<XF, WF, EXACT, DM_X_MX>(p, fm, fn, s);
+template <int XF, int WF, bool F32> int launch_src(const MxArgs& p, int x_src, int fm, int fn, hipStream_t s) {
+    if (x_src == DM_X_BF16) return launch_tile<XF, WF, F32, DM_X_BF16>(p, fm, fn, s);
+    if (x_src == DM_X_F32) return launch_tile<XF, WF, F32, DM_X_F32>(p, fm, fn, s);
+    return launch_tile<XF, WF, F32, DM_X_MX>(p, fm, fn, s);
 }
-template <int XF, int WF> int launch_exact(const MxArgs& p, bool exact, int x_src, int fm, int fn, hipStream_t s) {
-    if constexpr (XF == 8 || WF == 8)
-        if (exact) return launch_src<XF, WF, true>(p, x_src, fm, fn, s);
-    return launch_src<XF, WF, false>(p, x_src, fm, fn, s);
+template <int XF, int WF> int launch_result(const MxArgs& p, bool f32, int x_src, int fm, int fn, hipStream_t s) {
+    return f32 ? launch_src<XF, WF, true>(p, x_src, fm, fn, s) : launch_src<XF, WF, false>(p, x_src, fm, fn, s);
 }
 
 }  // namespace
 
-int dm_mx_split_launch(const MxArgs& p, int x_fmt, int w_fmt, bool exact, int x_src, int fm, int fn, hipStream_t stream) {
+int dm_mx_split_launch(const MxArgs& p, int x_fmt, int w_fmt, bool f32, int x_src, int fm, int fn, hipStream_t stream) {
     if (x_fmt == DM_MXFP8)
-        return w_fmt == DM_MXFP8 ? launch_exact<8, 8>(p, exact, x_src, fm, fn, stream) : launch_exact<8, 4>(p, exact, x_src, fm, fn, stream);
-    return w_fmt == DM_MXFP8 ? launch_exact<4, 8>(p, exact, x_src, fm, fn, stream) : launch_exact<4, 4>(p, exact, x_src, fm, fn, stream);
+        return w_fmt == DM_MXFP8 ? launch_result<8, 8>(p, f32, x_src, fm, fn, stream) : launch_result<8, 4>(p, f32, x_src, fm, fn, stream);
+    return w_fmt == DM_MXFP8 ? launch_result<4, 8>(p, f32, x_src, fm, fn, stream) : launch_result<4, 4>(p, f32, x_src, fm, fn, stream);
 }
