@@ -239,7 +239,7 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, *, x_format: str
     ``activation``: None, ``"quick_gelu"`` (v sigmoid(1.702 v)) or ``"geglu"`` (the first n / 2 columns times gelu(the others):
     ``[m, n / 2]``).  The result has ``out_dtype`` (bfloat16 / float32; ``residual`` has the same type), or is an
     :class:`MXTensor` with ``out_format`` (no residual).  Accumulation is fp32; bf16 and MX results come from the scaled matrix
-    instructions, which lose about 2e-5 of an 8-bit product.  fp32 results are fp32 sums of exact products, with activations right to a few
+    instructions, which lose about 2e-5 of an 8-bit product (where that matters, quantise or round an fp32 result).  fp32 results are fp32 sums of exact products, with activations right to a few
     units; for them an 8-bit operand's values are held in bf16, so those of scale bytes 0 to 2 are rounded to multiples of 2^-133 and those
     past bf16's largest (byte 247 on, which ``quantize`` never writes) are infinite."""
     what = "mx.linear"

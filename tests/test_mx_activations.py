@@ -11,7 +11,7 @@ from diffusion_model_amd import mx
 from test_mx_scale_offsets import _launches_tiles
 
 U = 2.0 ** -24
-N = 4096
+N = 4000
 
 
 def arguments(dev, low, high):
